@@ -275,6 +275,102 @@ int trb_add_rmsnorm(const void *x, const void *h, int32_t h_splits, const void *
 int trb_attn_prefill(const trb_cache_t *cache, const void *q, void *out, int32_t t, int32_t hq,
                      int64_t pos, float scale, trb_stream_t stream);
 
+/* ------------------------------------------------------------------ batches over a paged cache
+ * No counterpart in the reference (it serves one sequence).  K and V rows of many sequences lie in
+ * pages of one pool; a sequence is a row of a page table and a length on the device.  Sequences
+ * may share a prefix: prefix pages hold positions 0..P-1, a sequence's own pages hold positions
+ * P, P+1, ..  lens[b] = own rows of sequence b before the rows of this step; lens[b] < 0: the slot
+ * is empty (nothing is written for it, its attention output is zero).
+ *
+ * One layer's pool: k, v [num_pages, hkv, page_size, d] contiguous, scales [num_pages, hkv, page_size]. */
+typedef struct trb_paged {
+    void   *k, *v;
+    float  *k_scale, *v_scale;   /* NULL for a bf16 pool; positive and finite for live rows    */
+    int32_t hkv, d;              /* d in {128, 256}                                            */
+    int32_t kv_dtype;            /* TRB_KV_BF16 or TRB_KV_FP8                                  */
+    int32_t page_size;           /* rows per page: a power of two, 16 .. 65536                 */
+    int64_t num_pages;
+} trb_paged_t;
+
+/* The sequences of a step.  A page index outside the pool and a length beyond the table are recorded as
+ * TRB_ST_CURSOR_RANGE; their rows are neither written nor read. */
+typedef struct trb_batch {
+    const int32_t *table;        /* [n_seqs, table_pages], rows table_stride entries apart     */
+    int64_t     table_stride;
+    const void *lens;            /* [n_seqs] int32 or int64                                    */
+    int32_t     lens_width;      /* 4 or 8                                                     */
+    int32_t     n_seqs;          /* <= 1024                                                    */
+    int32_t     table_pages;
+    int32_t     reserved;
+} trb_batch_t;
+
+/* Append of the step's rows, with the norm and the rotation applied on the way.  Row t of q / k / v (bf16; element
+ * (row t, head h, dim x) at t * row_stride + h * head_stride + x) is row t - cu[b] of sequence b (cu NULL: t = b *
+ * rows_per_seq + i); it becomes own row lens[b] + i, position base + lens[b] + i.  q_norm_w / k_norm_w (optional):
+ * RMSNorm of each head with the (1 + w) gain.  Rotation of the first rotary_dim dims by position * inv_freq[pair]
+ * (computed in 64 bits), cos and sin times `amplitude`; pairs are (x, x + rotary_dim / 2) or, interleaved, (2x, 2x + 1).
+ * Everything is held in fp32 and rounded once: q_out to bf16, K and V to bf16 or to e4m3 codes with the scale max(amax, 1e-6) / 448.
+ * Rows at or beyond cu[n_seqs] and rows of empty slots write no cache row, and zeros to q_out. */
+typedef struct trb_paged_append_args {
+    const void *q, *k, *v;       /* q NULL: no query rows                                       */
+    void       *q_out;           /* [n_rows, hq, d] bf16                                        */
+    int64_t     q_row_stride, q_head_stride, k_row_stride, k_head_stride, v_row_stride, v_head_stride;
+    const void *q_norm_w, *k_norm_w;   /* [d] bf16 or NULL                                      */
+    const double *inv_freq;      /* [rotary_dim / 2] radians per position; NULL when rotary_dim is 0 */
+    const int32_t *cu;           /* [n_seqs + 1] first row of each sequence, or NULL            */
+    int32_t     n_rows, rows_per_seq, hq, rotary_dim, interleaved;
+    float       eps, amplitude;
+    trb_cursor_t base;           /* position of own row 0: the length of the shared prefix      */
+} trb_paged_append_args_t;
+int trb_paged_append(const trb_paged_t *pool, const trb_batch_t *batch, const trb_paged_append_args_t *args, trb_stream_t stream);
+
+/* Attention of the m new rows of every sequence (already appended): row i of sequence b sees all rows of the prefix
+ * and its own rows <= lens[b] + i.  A prefix that pays for it is read once for the whole batch, on the tensor
+ * cores.  New rows should be finite: a non-finite V row can reach the sequence's earlier rows of the same step.
+ * Rows of the pool that no query sees may hold anything.  (hq / hkv) * m <= 128. */
+typedef struct trb_attn_paged_args {
+    const void *q;               /* [n_seqs, m, hq, d] bf16                                     */
+    void       *out;             /* [n_seqs, m, hq, d] bf16                                     */
+    const void *gate;            /* optional, as in trb_decode_args: row = b * m + i            */
+    int64_t     gate_row_stride, gate_head_stride;
+    int32_t     m, hq;
+    float       scale;           /* softmax scale                                               */
+    int32_t     prefix_pages;    /* entries of prefix_table (0: no prefix)                      */
+    const int32_t *prefix_table;
+    trb_cursor_t prefix_len;     /* rows of the prefix                                          */
+    void       *workspace;       /* trb_attn_paged_workspace_bytes() bytes, any contents        */
+    size_t      workspace_bytes;
+} trb_attn_paged_args_t;
+size_t trb_attn_paged_workspace_bytes(const trb_paged_t *pool, int32_t n_seqs, int32_t m, int32_t hq, int32_t prefix_pages);
+int trb_attn_paged(const trb_paged_t *pool, const trb_batch_t *batch, const trb_attn_paged_args_t *args, trb_stream_t stream);
+
+/* Verification of drafted tokens by sampling, the counterpart of trb_spec_commit for a batch that does not decode
+ * greedily.  Draft i of sequence b (token x) is accepted while u[b][i] * q_i(x) < p_i(x); after the first rejection the
+ * new token is drawn from max(p_i - q_i, 0), after k acceptances from p_k, as the lowest index whose running sum
+ * exceeds u[b][k] times the total.  Products and sums are held in 64 bits.  draft_probs NULL: drafts were
+ * certain (q_i(x) = 1).  Entries that are not positive and finite count as zero; a residual without mass is replaced by
+ * p_i; a row without any mass gives token -1; a draft outside the vocabulary has probability zero.
+ * n_drafts (optional): drafts of each sequence, 0..k; negative: an empty slot (tokens -1, n_accepted 0).
+ * lens (optional): lens[b] += n_accepted + 1 for slots in use with lens[b] >= 0. */
+#define TRB_DT_F32  0
+#define TRB_DT_BF16 1
+#define TRB_DT_F16  2
+typedef struct trb_spec_verify_args {
+    const void *probs;           /* [n_seqs, k + 1, vocab], the last dim contiguous, rows probs_row_stride apart,
+                                    sequences probs_seq_stride apart (elements)                 */
+    const void *draft_probs;     /* [n_seqs, k, vocab] likewise, or NULL                        */
+    int64_t     probs_seq_stride, probs_row_stride, draft_seq_stride, draft_row_stride;
+    const int64_t *drafts;       /* [n_seqs, k]                                                 */
+    const float *u;              /* [n_seqs, k + 1] numbers in [0, 1)                           */
+    const int32_t *n_drafts;     /* [n_seqs] or NULL                                            */
+    int64_t    *tokens;          /* [n_seqs, k + 1]: accepted drafts, the new token, then -1    */
+    int64_t    *n_accepted;      /* [n_seqs]                                                    */
+    void       *lens;            /* [n_seqs] or NULL                                            */
+    int32_t     lens_width, n_seqs, k, vocab, dtype;   /* k <= 64                               */
+    int32_t     reserved;
+} trb_spec_verify_args_t;
+int trb_spec_verify(const trb_spec_verify_args_t *args, trb_stream_t stream);
+
 /* ------------------------------------------------------------------ sequence shards over NVLink
  * No counterpart in the reference (it is single-GPU); the math is its split merge
  * (tokenrush/fused.py:432-438) applied to one partial per GPU.

@@ -12,6 +12,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("TRB_KV_LIB") or os.path.join(HERE, "libtrb_kv.so")
 
 TRB_KV_BF16, TRB_KV_FP8 = 0, 1
+TRB_DT_F32, TRB_DT_BF16, TRB_DT_F16 = 0, 1, 2
 ST_CURSOR_RANGE, ST_WAIT_TIMEOUT, ST_PEER_TIMEOUT, ST_WORKSPACE = 1, 2, 4, 8
 IPC_HANDLE_BYTES = 64
 
@@ -52,6 +53,40 @@ class P2PMergeArgs(C.Structure):
                 ("gate_row_stride", C.c_int64), ("gate_head_stride", C.c_int64)]
 
 
+class Paged(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+                ("hkv", C.c_int32), ("d", C.c_int32), ("kv_dtype", C.c_int32), ("page_size", C.c_int32), ("num_pages", C.c_int64)]
+
+
+class Batch(C.Structure):
+    _fields_ = [("table", C.c_void_p), ("table_stride", C.c_int64), ("lens", C.c_void_p), ("lens_width", C.c_int32),
+                ("n_seqs", C.c_int32), ("table_pages", C.c_int32), ("reserved", C.c_int32)]
+
+
+class PagedAppendArgs(C.Structure):
+    _fields_ = [("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("q_out", C.c_void_p),
+                ("q_row_stride", C.c_int64), ("q_head_stride", C.c_int64), ("k_row_stride", C.c_int64),
+                ("k_head_stride", C.c_int64), ("v_row_stride", C.c_int64), ("v_head_stride", C.c_int64),
+                ("q_norm_w", C.c_void_p), ("k_norm_w", C.c_void_p), ("inv_freq", C.c_void_p), ("cu", C.c_void_p),
+                ("n_rows", C.c_int32), ("rows_per_seq", C.c_int32), ("hq", C.c_int32), ("rotary_dim", C.c_int32),
+                ("interleaved", C.c_int32), ("eps", C.c_float), ("amplitude", C.c_float), ("base", Cursor)]
+
+
+class AttnPagedArgs(C.Structure):
+    _fields_ = [("q", C.c_void_p), ("out", C.c_void_p), ("gate", C.c_void_p), ("gate_row_stride", C.c_int64),
+                ("gate_head_stride", C.c_int64), ("m", C.c_int32), ("hq", C.c_int32), ("scale", C.c_float),
+                ("prefix_pages", C.c_int32), ("prefix_table", C.c_void_p), ("prefix_len", Cursor),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+
+
+class SpecVerifyArgs(C.Structure):
+    _fields_ = [("probs", C.c_void_p), ("draft_probs", C.c_void_p), ("probs_seq_stride", C.c_int64),
+                ("probs_row_stride", C.c_int64), ("draft_seq_stride", C.c_int64), ("draft_row_stride", C.c_int64),
+                ("drafts", C.c_void_p), ("u", C.c_void_p), ("n_drafts", C.c_void_p), ("tokens", C.c_void_p),
+                ("n_accepted", C.c_void_p), ("lens", C.c_void_p), ("lens_width", C.c_int32), ("n_seqs", C.c_int32),
+                ("k", C.c_int32), ("vocab", C.c_int32), ("dtype", C.c_int32), ("reserved", C.c_int32)]
+
+
 # symbol -> (restype, argtypes); every function include/trb_kv.h declares
 SIGNATURES = {
     "trb_version": (C.c_int, []),
@@ -79,6 +114,10 @@ SIGNATURES = {
                                   C.c_void_p, C.c_void_p]),
     "trb_attn_prefill": (C.c_int, [C.POINTER(Cache), C.c_void_p, C.c_void_p, C.c_int32, C.c_int32, C.c_int64, C.c_float,
                                    C.c_void_p]),
+    "trb_paged_append": (C.c_int, [C.POINTER(Paged), C.POINTER(Batch), C.POINTER(PagedAppendArgs), C.c_void_p]),
+    "trb_attn_paged_workspace_bytes": (C.c_size_t, [C.POINTER(Paged), C.c_int32, C.c_int32, C.c_int32, C.c_int32]),
+    "trb_attn_paged": (C.c_int, [C.POINTER(Paged), C.POINTER(Batch), C.POINTER(AttnPagedArgs), C.c_void_p]),
+    "trb_spec_verify": (C.c_int, [C.POINTER(SpecVerifyArgs), C.c_void_p]),
     "trb_p2p_create": (C.c_int, [C.c_size_t, C.POINTER(C.c_void_p), C.c_void_p]),
     "trb_p2p_open": (C.c_int, [C.c_void_p, C.POINTER(C.c_void_p)]),
     "trb_p2p_close": (C.c_int, [C.c_void_p]),

@@ -246,6 +246,9 @@ int pdl_plan_decode(cudaStream_t st, const void *cache_k, const trb_cursor_t *po
                     const WrittenRange (&out)[3], const void *workspace, AppendSource *fresh);
 // an ordinary launch of the library on `st`: everything before it completes before anything after it starts
 void pdl_note_fence(cudaStream_t st);
+// a library launch that waits for everything before it at its top (and is counted by launch_kernel): the launches before
+// it are no longer in flight for the ones that follow
+void pdl_forget(cudaStream_t st);
 
 // Host: launch with (or without) the programmatic-stream-serialization attribute.
 inline bool pdl_enabled() { return pdl_mode() != 0; }

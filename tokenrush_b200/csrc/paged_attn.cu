@@ -1,0 +1,634 @@
+// Attention of a batch of sequences over a shared prefix and each sequence's own pages.
+//
+//   o = sum_x exp(s_x - m) v_x / sum_x exp(s_x - m),   s_x = scale q . k_x,   x over the prefix rows and the own rows <= lens[b] + i
+//
+// paged_scan_kernel reads cache rows for the few query rows of one sequence (G = hq / hkv heads x m tokens per kv
+// head) and is bound by HBM: the work is cut along one line of key tiles that runs through all sequences, every CTA
+// takes an equal piece of it whatever the lengths are, and a piece that covers part of a sequence leaves a (max, sum,
+// acc) partial that paged_merge_kernel joins.  The lengths are device integers: every CTA finds its piece itself.
+//
+// Inside a CTA four warps work on key tiles of their own, with a private ring of stages filled by cp.async: no
+// barrier is passed while tiles stream.  A tile is 16 keys, so it lies in one page, and 16 rows of a page are
+// contiguous.  The products run with the keys (resp. the head dims) as the 16-row operand of mma.m16n8k16 and the
+// query rows as the 8 columns, as in the contiguous decode kernel:
+//   S^T[16 keys x 8] = K Q^T,   O^T[dims x 8] += V^T P^T.
+// The order of dims inside a contraction is free, so a lane reads 16-byte chunks of a row (swizzled against bank
+// conflicts) instead of fragments, and the chunk's order is carried by how Q is laid out and O is read back.  e4m3 codes become f16 in
+// registers; the K scale multiplies the score, the V scale moves into the exponent, so codes are never scaled.
+#include "paged.cuh"
+
+namespace trb {
+
+constexpr int PS_WARPS = 4, PS_THREADS = PS_WARPS * 32, PS_STAGES = 3;
+
+struct PagedAttnParams {
+    PagedView c;
+    BatchView b;
+    const __nv_bfloat16 *q;
+    __nv_bfloat16 *out;
+    const __nv_bfloat16 *gate;
+    long long gate_rs, gate_hs;
+    int m, hq, g;                      // g = hq / hkv
+    float scale_log2;
+    const int *prefix_table;
+    int prefix_pages;                  // rows of the prefix that the scan itself reads come from here (0: none)
+    Cursor prefix_len;
+    int ctas;                          // CTAs per (kv head, row group)
+    int groups;                        // groups of 8 * NS query rows
+    int *plan;                         // [n_seqs][2]: first and last CTA with keys of the sequence
+    float *part_ml;                    // [hkv * groups][ctas + n_seqs][8 NS][2]
+    float *part_acc;                   // [hkv * groups][ctas + n_seqs][8 NS][D]
+};
+
+__device__ __forceinline__ void cp_async_16(uint32_t dst, const void *src, uint32_t src_bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(src_bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ uint4 ld_shared_v4(uint32_t a) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
+    return v;
+}
+
+// Rows of the prefix, and rows of one sequence's own pages, that this step may see (clamped to what the tables hold).
+__device__ __forceinline__ int paged_prefix_rows(const Cursor &len, int pages, int page_shift, bool report) {
+    long long n = pages > 0 ? load_cursor(len) : 0;
+    const long long most = (long long)pages << page_shift;
+    if (n < 0 || n > most) {
+        if (report) raise_status(TRB_ST_CURSOR_RANGE);
+        n = n < 0 ? 0 : most;
+    }
+    return (int)n;
+}
+__device__ __forceinline__ int paged_own_rows(const BatchView &b, int seq, int m, int page_shift, bool report) {
+    const long long len = load_len(b, seq);
+    if (len < 0) return -1;                                            // an empty slot
+    const long long most = (long long)b.table_pages << page_shift;
+    if (len + m > most) {
+        if (report) raise_status(TRB_ST_CURSOR_RANGE);
+        return (int)most;
+    }
+    return (int)(len + m);
+}
+
+template <int D_, bool FP8_, int NS_> struct ScanCfg {
+    static constexpr int D = D_, NS = NS_, SUB = D_ == 128 ? 2 : 1;     // 16-key tiles per pipeline step: 4 KB of K for e4m3, 8 KB for bf16
+    static constexpr bool FP8 = FP8_;
+    static constexpr int ROWB = D * (FP8 ? 1 : 2), CPR = ROWB / 16;    // bytes and 16-byte chunks of a row
+    static constexpr int TILE = 16 * ROWB, STAGE = SUB * 2 * TILE;
+    static constexpr int SC = FP8 ? SUB * 128 : 0;                     // scales of a stage: 16 K, 16 V per tile
+    static constexpr int RING = PS_STAGES * (STAGE + SC);
+    static constexpr int KJ = CPR / 4, VC = CPR / 8;                   // chunks per lane of a K row, of a V row
+    static constexpr int KS = D / 16;                                  // MMA steps of a QK product = row tiles of a PV product
+    static constexpr int OFF_Q = PS_WARPS * RING;                      // [NS][KS][32] uint2
+    static constexpr int OFF_QINV = OFF_Q + NS * KS * 256;             // [8 NS] floats
+    static constexpr int OFF_ML = OFF_QINV + NS * 32;                  // [warps][8 NS][2] floats
+    static constexpr int OFF_CNT = OFF_ML + PS_WARPS * NS * 64;        // [PG_MAX_SEQS + 1] ints, then 8 for the scan
+    static constexpr int SMEM = OFF_CNT + (PG_MAX_SEQS + 16) * 4;
+    static_assert(NS * 8 * D * 4 <= RING, "a warp's accumulators are exchanged through its ring");
+};
+
+template <typename C>
+__global__ void __launch_bounds__(PS_THREADS) paged_scan_kernel(const PagedAttnParams p) {
+    constexpr int D = C::D, NS = C::NS, SUB = C::SUB, KS = C::KS, KJ = C::KJ, VC = C::VC, CPR = C::CPR;
+    constexpr bool FP8 = C::FP8;
+    extern __shared__ __align__(128) uint8_t ps_smem[];
+    float *sm_qinv = reinterpret_cast<float *>(ps_smem + C::OFF_QINV);
+    float *sm_ml = reinterpret_cast<float *>(ps_smem + C::OFF_ML);
+    int *sm_cnt = reinterpret_cast<int *>(ps_smem + C::OFF_CNT);
+    uint2 *sm_q = reinterpret_cast<uint2 *>(ps_smem + C::OFF_Q);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int j = blockIdx.y % p.c.hkv, grp = blockIdx.y / p.c.hkv, hg = blockIdx.y;
+    const int rows = p.g * p.m, r0 = grp * 8 * NS;
+    const uint32_t ring = smem_u32(ps_smem + warp * C::RING);
+    pdl_wait();
+    pdl_launch_dependents();
+
+    // ---- the line of pipeline steps: sm_cnt[b] = steps before sequence b
+    const bool report = blockIdx.x == 0 && blockIdx.y == 0;
+    const int n_prefix = paged_prefix_rows(p.prefix_len, p.prefix_pages, p.c.page_shift, report && threadIdx.x == 0);
+    const int prefix_tiles = (n_prefix + 15) >> 4;
+    const int per = (p.b.n_seqs + PS_THREADS - 1) / PS_THREADS;
+    {
+        const int b0 = threadIdx.x * per;
+        int sum = 0;
+        for (int b = b0; b < b0 + per && b < p.b.n_seqs; ++b) {
+            const int own = paged_own_rows(p.b, b, p.m, p.c.page_shift, report);
+            const int steps = own < 0 ? 0 : (prefix_tiles + ((own + 15) >> 4) + SUB - 1) / SUB;
+            sm_cnt[b] = sum;
+            sum += steps;
+        }
+        int inc = sum;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) { const int v = __shfl_up_sync(0xffffffffu, inc, o); if (lane >= o) inc += v; }
+        int *wsum = sm_cnt + PG_MAX_SEQS + 1;
+        if (lane == 31) wsum[warp] = inc;
+        __syncthreads();
+        int before = inc - sum;
+        for (int w = 0; w < warp; ++w) before += wsum[w];
+        for (int b = b0; b < b0 + per && b < p.b.n_seqs; ++b) sm_cnt[b] += before;
+        if (threadIdx.x == PS_THREADS - 1) sm_cnt[p.b.n_seqs] = before + sum;
+        __syncthreads();
+    }
+    const int total = sm_cnt[p.b.n_seqs];
+    // a CTA gets at least one step for each of its warps
+    const int active = max(1, min(p.ctas, (total + PS_WARPS - 1) / PS_WARPS));
+    if (report) {
+        for (int b = threadIdx.x; b < p.b.n_seqs; b += PS_THREADS) {
+            const int lo = sm_cnt[b], hi = sm_cnt[b + 1];
+            p.plan[2 * b] = hi > lo ? (int)((((long long)lo + 1) * active - 1) / total) : 0;      // the CTA that owns step lo
+            p.plan[2 * b + 1] = hi > lo ? (int)(((long long)hi * active - 1) / total) : -1;       // ... and step hi - 1
+        }
+    }
+    if ((int)blockIdx.x >= active || total == 0) return;
+    const int lo = (int)((long long)blockIdx.x * total / active), hi = (int)(((long long)blockIdx.x + 1) * total / active);
+    if (lo >= hi) return;
+    int seq;
+    {
+        int a = 0, z = p.b.n_seqs;                                      // last sequence that starts at or before lo
+        while (z - a > 1) { const int mid = (a + z) >> 1; if (sm_cnt[mid] <= lo) a = mid; else z = mid; }
+        seq = a;
+        while (sm_cnt[seq + 1] <= lo) ++seq;                            // (skips slots without steps that start at lo)
+    }
+
+    for (; seq < p.b.n_seqs && sm_cnt[seq] < hi; ++seq) {
+        const int s0 = max(lo, sm_cnt[seq]) - sm_cnt[seq], s1 = min(hi, sm_cnt[seq + 1]) - sm_cnt[seq];
+        if (s1 <= s0) continue;
+        const int own = paged_own_rows(p.b, seq, p.m, p.c.page_shift, false);
+        const long long len = load_len(p.b, seq);
+        const int *own_table = p.b.table + seq * p.b.table_stride;
+
+        // ---- pipeline of this warp: steps s0 + warp, s0 + warp + 4, ..
+        auto page_of = [&](int tile) -> int {                          // pool page of a tile, -1: none
+            const int x = tile - prefix_tiles;
+            int pg = -1;
+            if (x < 0) pg = p.prefix_table[(tile * 16) >> p.c.page_shift];
+            else if (x * 16 < own) pg = own_table[(x * 16) >> p.c.page_shift];
+            else return -1;
+            if (pg < 0 || pg >= p.c.num_pages) { if (lane == 0) raise_status(TRB_ST_CURSOR_RANGE); pg = -1; }
+            return pg;
+        };
+        auto load_step = [&](int step, int stage, const int (&pages)[SUB]) {
+            const uint32_t base = ring + stage * (C::STAGE + C::SC);
+#pragma unroll
+            for (int sb = 0; sb < SUB; ++sb) {
+                const int tile = step * SUB + sb, x = tile - prefix_tiles;
+                const int row = x < 0 ? tile * 16 : x * 16, limit = pages[sb] < 0 ? 0 : (x < 0 ? n_prefix : own);
+                const int left = limit - row;                          // rows of the tile that exist; the others are zero
+                const long long first = pages[sb] < 0 ? 0
+                                        : ((((long long)pages[sb] * p.c.hkv + j) << p.c.page_shift) + (row & ((1 << p.c.page_shift) - 1)));
+                const uint8_t *ks = p.c.k + first * C::ROWB + lane * 16, *vs = p.c.v + first * C::ROWB + lane * 16;
+                const uint32_t kd = base + sb * 2 * C::TILE, vd = kd + C::TILE;
+#pragma unroll
+                for (int i = 0; i < CPR / 2; ++i) {                    // 16 rows x CPR chunks over 32 lanes
+                    const int idx = i * 32 + lane, r = idx / CPR, ch = idx % CPR;
+                    const uint32_t n = r < left ? 16u : 0u;
+                    const uint32_t off = r < left ? i * 512 : 0;
+                    cp_async_16(kd + r * C::ROWB + ((ch ^ ((r & 1) << 2)) << 4), ks + off, n);
+                    cp_async_16(vd + r * C::ROWB + ((ch ^ (r & 6)) << 4), vs + off, n);
+                }
+                if constexpr (FP8) {
+                    const bool ok = (lane & 15) < left;
+                    const float *sc = (lane < 16 ? p.c.ks : p.c.vs) + first + (ok ? (lane & 15) : 0);
+                    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(base + C::STAGE + sb * 128 + lane * 4), "l"(sc), "r"(ok ? 4u : 0u) : "memory");
+                }
+            }
+            cp_async_commit();
+        };
+        const int steps = s1 - s0 > warp ? (s1 - s0 - warp + PS_WARPS - 1) / PS_WARPS : 0;
+        int pages[SUB];
+        auto fetch_pages = [&](int k) {
+#pragma unroll
+            for (int sb = 0; sb < SUB; ++sb) pages[sb] = k < steps ? page_of((s0 + warp + k * PS_WARPS) * SUB + sb) : -1;
+        };
+        fetch_pages(0);
+#pragma unroll
+        for (int k = 0; k < PS_STAGES - 1; ++k) {
+            int now[SUB];
+#pragma unroll
+            for (int sb = 0; sb < SUB; ++sb) now[sb] = pages[sb];
+            fetch_pages(k + 1);
+            if (k < steps) load_step(s0 + warp + k * PS_WARPS, k, now);
+            else cp_async_commit();
+        }
+
+        // ---- the query rows as MMA fragments: step (jj, w) of lane (g, t) holds dims of chunk 4 jj + t.  e4m3: f16 with a power-of-two
+        // factor for each row (a bf16 value may lie outside f16's range); bf16: as they are.
+        for (int s = warp; s < NS; s += PS_WARPS) {
+            const int r = r0 + s * 8 + g;
+            const bool ok = r < rows;
+            const __nv_bfloat16 *src = p.q + (((long long)seq * p.m + (ok ? r / p.g : 0)) * p.hq + j * p.g + (ok ? r % p.g : 0)) * D;
+            constexpr int DPC = FP8 ? 16 : 8;                           // dims of a chunk
+            float mult = 1.f;
+            if constexpr (FP8) {
+                float amax = 0.f;
+                for (int jj = 0; jj < KJ; ++jj)
+#pragma unroll
+                    for (int x = 0; x < DPC; ++x) amax = fmaxf(amax, fabsf(__bfloat162float(src[(4 * jj + t) * DPC + x])));
+                amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+                amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+                int e = (int)((__float_as_uint(amax) >> 23) & 0xffu) - 127;
+                e = amax == 0.f ? 0 : max(-90, min(90, e));
+                mult = __uint_as_float((uint32_t)(127 - e) << 23);
+                if (t == 0) sm_qinv[s * 8 + g] = __uint_as_float((uint32_t)(127 + e) << 23);
+            }
+            for (int jj = 0; jj < KJ; ++jj)
+#pragma unroll
+                for (int x = 0; x < DPC / 4; ++x) {
+                    const uint2 raw = *reinterpret_cast<const uint2 *>(src + (4 * jj + t) * DPC + x * 4);
+                    uint2 w = ok ? raw : make_uint2(0u, 0u);
+                    if constexpr (FP8) {
+                        const float2 a = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&w.x));
+                        const float2 b = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&w.y));
+                        w = make_uint2(pack_f16x2(a.x * mult, a.y * mult), pack_f16x2(b.x * mult, b.y * mult));
+                    }
+                    sm_q[(s * KS + jj * (DPC / 4) + x) * 32 + lane] = w;
+                }
+        }
+        __syncthreads();
+        uint2 qf[NS == 1 ? KS : 1];
+        if constexpr (NS == 1) {
+#pragma unroll
+            for (int x = 0; x < KS; ++x) qf[x] = sm_q[x * 32 + lane];
+        }
+        // this thread's query rows are columns 2t, 2t + 1 of each slice
+        float qinv[NS * 2], ref[NS * 2], l[NS * 2], acc[NS][KS][4];
+        int last[NS * 2];                                              // own rows below this are visible
+#pragma unroll
+        for (int s = 0; s < NS; ++s)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int r = r0 + s * 8 + 2 * t + e;
+                qinv[s * 2 + e] = FP8 ? sm_qinv[s * 8 + 2 * t + e] * p.scale_log2 : p.scale_log2;
+                last[s * 2 + e] = (int)min((long long)own, len + 1 + (r < rows ? r / p.g : p.m));
+                ref[s * 2 + e] = -INFINITY;
+                l[s * 2 + e] = 0.f;
+            }
+#pragma unroll
+        for (int s = 0; s < NS; ++s)
+#pragma unroll
+            for (int a = 0; a < KS; ++a)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[s][a][e] = 0.f;
+
+        for (int k = 0; k < steps; ++k) {
+            {                                                          // request the step PS_STAGES - 1 ahead
+                int now[SUB];
+#pragma unroll
+                for (int sb = 0; sb < SUB; ++sb) now[sb] = pages[sb];
+                fetch_pages(k + PS_STAGES);
+                if (k + PS_STAGES - 1 < steps) load_step(s0 + warp + (k + PS_STAGES - 1) * PS_WARPS, (k + PS_STAGES - 1) % PS_STAGES, now);
+                else cp_async_commit();
+            }
+            cp_async_wait<PS_STAGES - 1>();
+            __syncwarp();
+            const uint32_t base = ring + (k % PS_STAGES) * (C::STAGE + C::SC);
+            const int step = s0 + warp + k * PS_WARPS;
+
+            // S^T: two chains of MMAs per tile
+            float sc[SUB][NS][4];
+#pragma unroll
+            for (int sb = 0; sb < SUB; ++sb) {
+                float s2[NS][2][4];
+#pragma unroll
+                for (int s = 0; s < NS; ++s)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s2[s][0][e] = s2[s][1][e] = 0.f;
+                const uint32_t kb = base + sb * 2 * C::TILE + g * C::ROWB;
+#pragma unroll
+                for (int jj = 0; jj < KJ; ++jj) {
+                    const uint32_t ch = ((4 * jj + t) ^ ((g & 1) << 2)) << 4;
+                    const uint4 x = ld_shared_v4(kb + ch), y = ld_shared_v4(kb + 8 * C::ROWB + ch);
+                    const uint32_t xw[4] = {x.x, x.y, x.z, x.w}, yw[4] = {y.x, y.y, y.z, y.w};
+                    if constexpr (FP8) {
+#pragma unroll
+                        for (int w = 0; w < 4; ++w) {
+                            const uint32_t a[4] = {e4m3x2_to_f16x2((uint16_t)xw[w]), e4m3x2_to_f16x2((uint16_t)yw[w]),
+                                                   e4m3x2_to_f16x2((uint16_t)(xw[w] >> 16)), e4m3x2_to_f16x2((uint16_t)(yw[w] >> 16))};
+#pragma unroll
+                            for (int s = 0; s < NS; ++s) {
+                                const uint2 b = NS == 1 ? qf[jj * 4 + w] : sm_q[(s * KS + jj * 4 + w) * 32 + lane];
+                                mma_f16(s2[s][w & 1], a, b.x, b.y);
+                            }
+                        }
+                    } else {
+#pragma unroll
+                        for (int w = 0; w < 2; ++w) {
+                            const uint32_t a[4] = {xw[2 * w], yw[2 * w], xw[2 * w + 1], yw[2 * w + 1]};
+#pragma unroll
+                            for (int s = 0; s < NS; ++s) {
+                                const uint2 b = NS == 1 ? qf[jj * 2 + w] : sm_q[(s * KS + jj * 2 + w) * 32 + lane];
+                                mma_bf16(s2[s][w], a, b.x, b.y);
+                            }
+                        }
+                    }
+                }
+#pragma unroll
+                for (int s = 0; s < NS; ++s)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) sc[sb][s][e] = s2[s][0][e] + s2[s][1][e];
+            }
+            // scores in log2 units (+ log2 of the V scale), masked; element e: key g + 8 (e >> 1), column 2t + (e & 1)
+            float vinv[SUB][2];
+            bool raise = false;
+#pragma unroll
+            for (int sb = 0; sb < SUB; ++sb) {
+                float kf[2] = {1.f, 1.f}, vl[2] = {0.f, 0.f};
+                if constexpr (FP8) {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        float kk, vv;
+                        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(kk) : "r"(base + C::STAGE + sb * 128 + (g + 8 * h) * 4));
+                        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(vv) : "r"(base + C::STAGE + sb * 128 + 64 + (g + 8 * h) * 4));
+                        kf[h] = kk;
+                        vl[h] = __log2f(vv);
+                        vinv[sb][h] = __fdividef(1.f, vv);
+                    }
+                }
+                const int tile = step * SUB + sb, x = tile - prefix_tiles;
+                const int row = x < 0 ? tile * 16 : x * 16;
+#pragma unroll
+                for (int s = 0; s < NS; ++s)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float v = FP8 ? fmaf(sc[sb][s][e] * kf[e >> 1], qinv[s * 2 + (e & 1)], vl[e >> 1]) : sc[sb][s][e] * qinv[s * 2 + (e & 1)];
+                        const int limit = x < 0 ? n_prefix : last[s * 2 + (e & 1)];
+                        sc[sb][s][e] = row + g + 8 * (e >> 1) < limit ? v : -INFINITY;
+                        raise |= sc[sb][s][e] > ref[s * 2 + (e & 1)] + 8.f;
+                    }
+            }
+            // the reference of a row follows its maximum lazily: weights up to 2^8 fit f16, so it moves only when a score
+            // passes it by more
+            if (__any_sync(0xffffffffu, raise)) {
+#pragma unroll
+                for (int s = 0; s < NS; ++s)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        float mx = -INFINITY;
+#pragma unroll
+                        for (int sb = 0; sb < SUB; ++sb) mx = fmaxf(mx, fmaxf(sc[sb][s][e], sc[sb][s][e + 2]));
+                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+                        mx = fmaxf(mx, ref[s * 2 + e]);
+                        const float alpha = mx == -INFINITY ? 1.f : fast_exp2(ref[s * 2 + e] - mx);
+                        ref[s * 2 + e] = mx;
+                        l[s * 2 + e] *= alpha;
+#pragma unroll
+                        for (int a = 0; a < KS; ++a) { acc[s][a][e] *= alpha; acc[s][a][e + 2] *= alpha; }
+                    }
+            }
+            // weights and O^T += V^T P^T
+#pragma unroll
+            for (int sb = 0; sb < SUB; ++sb) {
+                uint32_t pb[NS][2];
+#pragma unroll
+                for (int s = 0; s < NS; ++s) {
+                    float w[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float m0 = ref[s * 2 + (e & 1)];
+                        w[e] = fast_exp2(sc[sb][s][e] - (m0 == -INFINITY ? 0.f : m0));
+                    }
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        uint32_t pk;
+                        if constexpr (FP8) {
+                            pk = pack_f16x2(w[2 * h], w[2 * h + 1]);
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) l[s * 2 + e] += w[2 * h + e] > 0.f ? w[2 * h + e] * vinv[sb][h] : w[2 * h + e] * 0.f;
+                        } else {
+                            // the sum takes the weights as they multiply V
+                            pk = pack_bf16x2(w[2 * h], w[2 * h + 1]);
+                            const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&pk));
+                            l[s * 2] += f.x;
+                            l[s * 2 + 1] += f.y;
+                        }
+                        pb[s][h] = movmatrix_trans(pk);
+                    }
+                }
+                const uint32_t vb = base + sb * 2 * C::TILE + C::TILE + 2 * t * C::ROWB;
+#pragma unroll
+                for (int c = 0; c < VC; ++c) {
+                    // keys 2t, 2t + 1, 2t + 8, 2t + 9: rows of equal (row & 6) = 2t & 6
+                    const uint32_t ch = ((g + 8 * c) ^ ((2 * t) & 6)) << 4;
+                    uint4 v[4] = {ld_shared_v4(vb + ch), ld_shared_v4(vb + C::ROWB + ch), ld_shared_v4(vb + 8 * C::ROWB + ch), ld_shared_v4(vb + 9 * C::ROWB + ch)};
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) {
+                        const uint32_t k0 = w == 0 ? v[0].x : w == 1 ? v[0].y : w == 2 ? v[0].z : v[0].w;
+                        const uint32_t k1 = w == 0 ? v[1].x : w == 1 ? v[1].y : w == 2 ? v[1].z : v[1].w;
+                        const uint32_t k2 = w == 0 ? v[2].x : w == 1 ? v[2].y : w == 2 ? v[2].z : v[2].w;
+                        const uint32_t k3 = w == 0 ? v[3].x : w == 1 ? v[3].y : w == 2 ? v[3].z : v[3].w;
+                        if constexpr (FP8) {
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) {
+                                const uint32_t x01 = prmt(k0, k1, h ? 0x7362 : 0x5140), x23 = prmt(k2, k3, h ? 0x7362 : 0x5140);
+                                const uint32_t a[4] = {e4m3x2_to_f16x2((uint16_t)x01), e4m3x2_to_f16x2((uint16_t)(x01 >> 16)),
+                                                       e4m3x2_to_f16x2((uint16_t)x23), e4m3x2_to_f16x2((uint16_t)(x23 >> 16))};
+#pragma unroll
+                                for (int s = 0; s < NS; ++s) mma_f16(acc[s][c * 8 + w * 2 + h], a, pb[s][0], pb[s][1]);
+                            }
+                        } else {
+                            const uint32_t a[4] = {prmt(k0, k1, 0x5410), prmt(k0, k1, 0x7632), prmt(k2, k3, 0x5410), prmt(k2, k3, 0x7632)};
+#pragma unroll
+                            for (int s = 0; s < NS; ++s) mma_bf16(acc[s][c * 4 + w], a, pb[s][0], pb[s][1]);
+                        }
+                    }
+                }
+            }
+            __syncwarp();                                              // the stage may be refilled
+        }
+        cp_async_wait<0>();
+        __syncwarp();
+
+        // ---- join the four warps through their rings and write the piece's partial
+#pragma unroll
+        for (int x = 0; x < NS * 2; ++x) {
+            l[x] += __shfl_xor_sync(0xffffffffu, l[x], 4);
+            l[x] += __shfl_xor_sync(0xffffffffu, l[x], 8);
+            l[x] += __shfl_xor_sync(0xffffffffu, l[x], 16);
+            if (g == 0) {
+                float *ml = sm_ml + (warp * 8 * NS + (x >> 1) * 8 + 2 * t + (x & 1)) * 2;
+                ml[0] = ref[x];
+                ml[1] = l[x];
+            }
+        }
+        // a lane's accumulators as 16-byte pieces of consecutive dims: [slice][column parity][chunk c][piece f]
+        constexpr int PIECES = (FP8 ? 16 : 8) / 4, QUADS = 2 * VC * PIECES;
+        float4 *red = reinterpret_cast<float4 *>(ps_smem + warp * C::RING);
+#pragma unroll
+        for (int s = 0; s < NS; ++s)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+#pragma unroll
+                for (int c = 0; c < VC; ++c)
+#pragma unroll
+                    for (int f = 0; f < PIECES; ++f) {
+                        const int a = c * 2 * PIECES + f * 2;          // two row tiles hold four consecutive dims
+                        red[(s * QUADS + (e * VC + c) * PIECES + f) * 32 + lane] = make_float4(acc[s][a][e], acc[s][a][e + 2], acc[s][a + 1][e], acc[s][a + 1][e + 2]);
+                    }
+        __syncthreads();
+        const long long slot = (long long)hg * (p.ctas + p.b.n_seqs) + blockIdx.x + seq;
+        for (int x = warp; x < NS * QUADS; x += PS_WARPS) {
+            const int s = x / QUADS, e = (x / (VC * PIECES)) & 1, c = (x / PIECES) % VC, f = x % PIECES;
+            const int col = s * 8 + 2 * t + e;
+            float m4[PS_WARPS], mx = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < PS_WARPS; ++w) { m4[w] = sm_ml[(w * 8 * NS + col) * 2]; mx = fmaxf(mx, m4[w]); }
+            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+            float lt = 0.f;
+#pragma unroll
+            for (int w = 0; w < PS_WARPS; ++w) {
+                const float al = m4[w] == -INFINITY ? 0.f : fast_exp2(m4[w] - mx);
+                const float4 v = reinterpret_cast<const float4 *>(ps_smem + w * C::RING)[x * 32 + lane];
+                o.x = fmaf(v.x, al, o.x); o.y = fmaf(v.y, al, o.y); o.z = fmaf(v.z, al, o.z); o.w = fmaf(v.w, al, o.w);
+                lt = fmaf(sm_ml[(w * 8 * NS + col) * 2 + 1], al, lt);
+            }
+            if (r0 + col < rows) {
+                const int dim = (g + 8 * c) * (FP8 ? 16 : 8) + f * 4;
+                *reinterpret_cast<float4 *>(p.part_acc + (slot * 8 * NS + col) * D + dim) = o;
+                if (c == 0 && f == 0 && g == 0) *reinterpret_cast<float2 *>(p.part_ml + (slot * 8 * NS + col) * 2) = make_float2(mx, lt);
+            }
+        }
+        __syncthreads();
+    }
+}
+
+// Joins the partials of a query row, one warp per row: at most plan[1] - plan[0] + 1 pieces of the scan.  The weights
+// exp2(m - max) are found 32 pieces at a time, one per lane.  Latency-bound: a few KB per row, all from L2.
+template <int D>
+__global__ void __launch_bounds__(256) paged_merge_kernel(const PagedAttnParams p, const int ns) {
+    constexpr int EPT = D / 32;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const long long row = (long long)blockIdx.x * 8 + warp;                // (sequence, token, head)
+    pdl_wait();
+    pdl_launch_dependents();
+    if (row >= (long long)p.b.n_seqs * p.m * p.hq) return;
+    const int h = (int)(row % p.hq), i = (int)(row / p.hq % p.m), seq = (int)(row / p.hq / p.m);
+    const int j = h / p.g, r = i * p.g + h % p.g, grp = r / (8 * ns), col = r % (8 * ns);
+    const int c0 = p.plan[2 * seq], c1 = p.plan[2 * seq + 1];
+    const long long slot0 = (long long)(grp * p.c.hkv + j) * (p.ctas + p.b.n_seqs) + seq;
+    float mx = -INFINITY, l = 0.f, o[EPT];
+#pragma unroll
+    for (int e = 0; e < EPT; ++e) o[e] = 0.f;
+    for (int base = c0; base <= c1; base += 32) {
+        const int n = min(32, c1 - base + 1);
+        float2 ml = make_float2(-INFINITY, 0.f);
+        if (lane < n) ml = *reinterpret_cast<const float2 *>(p.part_ml + ((slot0 + base + lane) * 8 * ns + col) * 2);
+        const float m_new = fmaxf(mx, warp_max(ml.x));
+        const float w = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - m_new);
+        const float alpha = mx == -INFINITY ? 0.f : fast_exp2(mx - m_new);
+        l = l * alpha + warp_sum(w == 0.f && ml.y == ml.y ? 0.f : ml.y * w);
+#pragma unroll
+        for (int e = 0; e < EPT; ++e) o[e] *= alpha;
+        mx = m_new;
+        for (int x = 0; x < n; ++x) {
+            const float wx = __shfl_sync(0xffffffffu, w, x);
+            const float4 *src = reinterpret_cast<const float4 *>(p.part_acc + ((slot0 + base + x) * 8 * ns + col) * D + lane * EPT);
+#pragma unroll
+            for (int e = 0; e < EPT / 4; ++e) {
+                const float4 v = src[e];
+                o[e * 4] = fmaf(v.x, wx, o[e * 4]); o[e * 4 + 1] = fmaf(v.y, wx, o[e * 4 + 1]);
+                o[e * 4 + 2] = fmaf(v.z, wx, o[e * 4 + 2]); o[e * 4 + 3] = fmaf(v.w, wx, o[e * 4 + 3]);
+            }
+        }
+    }
+    const float inv = l == 0.f ? 0.f : __fdiv_rn(1.f, l);                 // a row that sees no key is zero
+    __nv_bfloat16 ob[EPT];
+#pragma unroll
+    for (int e = 0; e < EPT; ++e) ob[e] = __float2bfloat16_rn(o[e] * inv);
+    if (p.gate) {
+        const __nv_bfloat16 *gp = p.gate + ((long long)seq * p.m + i) * p.gate_rs + h * p.gate_hs + lane * EPT;
+#pragma unroll
+        for (int e = 0; e < EPT; ++e) {
+            const __nv_bfloat16 sg = __float2bfloat16_rn(__fdiv_rn(1.f, 1.f + __expf(-__bfloat162float(gp[e]))));
+            ob[e] = __float2bfloat16_rn(__bfloat162float(ob[e]) * __bfloat162float(sg));
+        }
+    }
+    __nv_bfloat16 *dst = p.out + row * D + lane * EPT;
+    if (EPT == 8) *reinterpret_cast<uint4 *>(dst) = *reinterpret_cast<const uint4 *>(ob);
+    else *reinterpret_cast<uint2 *>(dst) = *reinterpret_cast<const uint2 *>(ob);
+}
+
+// How a call is cut: query-row slices per CTA, row groups, CTAs per (kv head, group), and where its partials lie.
+struct PagedAttnPlan {
+    int ns, groups, ctas;
+    size_t off_ml, off_acc, bytes;
+};
+static PagedAttnPlan paged_attn_plan(int d, bool fp8, int hkv, int hq, int n_seqs, int m) {
+    PagedAttnPlan o;
+    const int rows = hq / hkv * m;
+    o.ns = rows <= 8 ? 1 : 2;
+    o.groups = (rows + 8 * o.ns - 1) / (8 * o.ns);
+    const int per_sm = fp8 ? 2 : 1;                                       // CTAs that fit an SM (shared memory)
+    o.ctas = std::max(1, sm_count() * per_sm / (hkv * o.groups));
+    const size_t slots = (size_t)hkv * o.groups * (o.ctas + n_seqs) * 8 * o.ns;
+    o.off_ml = ((size_t)n_seqs * 8 + 255) / 256 * 256;
+    o.off_acc = (o.off_ml + slots * 8 + 255) / 256 * 256;
+    o.bytes = o.off_acc + slots * d * 4;
+    return o;
+}
+
+template <typename C>
+static int launch_scan(const PagedAttnParams &p, cudaStream_t st) {
+    static bool attr_set[64] = {};
+    int dev = 0;
+    TRB_CUDA_CHECK(cudaGetDevice(&dev));
+    if (!attr_set[dev & 63]) {
+        TRB_CUDA_CHECK(cudaFuncSetAttribute(paged_scan_kernel<C>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
+        attr_set[dev & 63] = true;
+    }
+    TRB_CUDA_CHECK(launch_kernel(paged_scan_kernel<C>, dim3(p.ctas, p.c.hkv * p.groups), dim3(PS_THREADS), C::SMEM, st, true, p));
+    return TRB_OK;
+}
+
+}  // namespace trb
+
+using namespace trb;
+
+static int check_paged_geometry(const trb_paged_t *pool, int n_seqs, int m, int hq, int prefix_pages) {
+    if (n_seqs < 1 || m < 1 || hq < 1 || prefix_pages < 0 || hq % pool->hkv) return TRB_E_ARG;
+    if (n_seqs > PG_MAX_SEQS || (long long)(hq / pool->hkv) * m > 128) return TRB_E_UNSUPPORTED;
+    return TRB_OK;
+}
+
+extern "C" size_t trb_attn_paged_workspace_bytes(const trb_paged_t *pool, int32_t n_seqs, int32_t m, int32_t hq, int32_t prefix_pages) {
+    PagedView v;
+    if (make_paged_view(pool, &v) || check_paged_geometry(pool, n_seqs, m, hq, prefix_pages)) return 0;
+    return paged_attn_plan(pool->d, v.ks != nullptr, pool->hkv, hq, n_seqs, m).bytes;
+}
+
+extern "C" int trb_attn_paged(const trb_paged_t *pool, const trb_batch_t *batch, const trb_attn_paged_args_t *a, trb_stream_t stream) {
+    PagedAttnParams p;
+    int rc = make_paged_view(pool, &p.c);
+    if (rc || (rc = make_batch_view(batch, &p.b))) return rc;
+    if (!a || !a->q || !a->out || !a->workspace || (a->prefix_pages > 0 && !a->prefix_table)) return TRB_E_ARG;
+    if ((rc = check_paged_geometry(pool, batch->n_seqs, a->m, a->hq, a->prefix_pages))) return rc;
+    if (a->prefix_pages > 0 && (rc = check_cursor(&a->prefix_len))) return rc;
+    // rows are counted in 32 bits, with room for a step of tiles behind the last one
+    if (((long long)a->prefix_pages + batch->table_pages) << p.c.page_shift > 0x7fffff00LL) return TRB_E_UNSUPPORTED;
+    if (((((long long)a->prefix_pages + batch->table_pages) << p.c.page_shift) / 16 + 2) * batch->n_seqs > 0x7fffffffLL) return TRB_E_UNSUPPORTED;
+    if ((((uintptr_t)a->q | (uintptr_t)a->out) & 15) || ((uintptr_t)a->workspace & 255) || ((uintptr_t)a->prefix_table & 3) || ((uintptr_t)a->gate & 1)) return TRB_E_ALIGN;
+    const bool fp8 = p.c.ks != nullptr;
+    const PagedAttnPlan plan = paged_attn_plan(pool->d, fp8, pool->hkv, a->hq, batch->n_seqs, a->m);
+    if (a->workspace_bytes < plan.bytes) return TRB_E_CAPACITY;
+    p.q = (const __nv_bfloat16 *)a->q; p.out = (__nv_bfloat16 *)a->out; p.gate = (const __nv_bfloat16 *)a->gate;
+    p.gate_rs = a->gate_row_stride; p.gate_hs = a->gate_head_stride;
+    p.m = a->m; p.hq = a->hq; p.g = a->hq / pool->hkv; p.scale_log2 = a->scale * 1.4426950408889634f;
+    p.prefix_table = a->prefix_table; p.prefix_pages = a->prefix_pages; p.prefix_len = make_cursor(&a->prefix_len);
+    p.ctas = plan.ctas; p.groups = plan.groups;
+    uint8_t *ws = (uint8_t *)a->workspace;
+    p.plan = (int *)ws; p.part_ml = (float *)(ws + plan.off_ml); p.part_acc = (float *)(ws + plan.off_acc);
+    cudaStream_t st = (cudaStream_t)stream;
+    pdl_forget(st);
+    if (plan.ns == 1) rc = pool->d == 256 ? (fp8 ? launch_scan<ScanCfg<256, true, 1>>(p, st) : launch_scan<ScanCfg<256, false, 1>>(p, st))
+                                          : (fp8 ? launch_scan<ScanCfg<128, true, 1>>(p, st) : launch_scan<ScanCfg<128, false, 1>>(p, st));
+    else rc = pool->d == 256 ? (fp8 ? launch_scan<ScanCfg<256, true, 2>>(p, st) : launch_scan<ScanCfg<256, false, 2>>(p, st))
+                             : (fp8 ? launch_scan<ScanCfg<128, true, 2>>(p, st) : launch_scan<ScanCfg<128, false, 2>>(p, st));
+    if (rc) return rc;
+    const long long out_rows = (long long)batch->n_seqs * a->m * a->hq;
+    TRB_CUDA_CHECK(launch_kernel(pool->d == 256 ? paged_merge_kernel<256> : paged_merge_kernel<128>, dim3((unsigned)((out_rows + 7) / 8)), dim3(256), 0, st,
+                                 true, p, plan.ns));
+    return TRB_OK;
+}

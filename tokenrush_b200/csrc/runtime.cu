@@ -152,6 +152,10 @@ void note_launch() { g_launches.fetch_add(1, std::memory_order_relaxed); }
 // complete when it runs (every such launch site calls this right before its one launch).
 void pdl_note_fence(cudaStream_t st) {
     note_launch();
+    pdl_forget(st);
+}
+
+void pdl_forget(cudaStream_t st) {
     std::lock_guard<std::mutex> lock(g_track_mu);
     auto it = g_track.find(st);
     if (it != g_track.end()) it->second.s.clear();

@@ -8,6 +8,8 @@ argument meaning, backed by the sm_100a CUDA library through its C ABI.
     attn_window_block    tokenrush/fused.py:600-622
     add_rmsnorm          tokenrush/fused.py:48-60    (the step after the attention output projection)
 
+For batches of sequences (the reference serves one) over a paged cache: `paged_append`, `attn_paged` and
+`spec_verify`, the batch's prep, decode and commit,
 plus the cursor arithmetic the reference does with small torch ops (`spec_commit`,
 tokenrush/model.py:306-312) and the ring write of the DFlash draft cache (`ring_write`,
 tokenrush/dflash.py:293-294).  Every call launches on torch's current stream, allocates
@@ -328,3 +330,172 @@ def cursor_advance(pos_t, delta: int):
     """pos_t += delta on the device, as one tiny launch (State.advance's device half)."""
     _need_cuda(pos_t)
     L.check(L.lib().trb_cursor_advance(pos_t.data_ptr(), pos_t.element_size(), int(delta), _stream()), "trb_cursor_advance")
+
+
+# ------------------------------------------------------------------------------ batches over a paged cache
+
+def _on_device(*ts) -> int:
+    """The index of the current device, which all the tensors given have to be on."""
+    for t in ts:
+        if t is not None and not t.is_cuda:
+            raise RuntimeError("tokenrush_b200 runs on CUDA tensors only (there is no CPU path)")
+    index = torch.cuda.current_device()
+    for t in ts:
+        if t is not None and t.get_device() != index:
+            raise RuntimeError(f"a tensor is on cuda:{t.get_device()}, the current device is cuda:{index}")
+    return index
+
+
+def _pool(k_pages, v_pages, k_scale, v_scale) -> L.Paged:
+    """One layer's pool of pages [PAGES, HKV, PAGE, D] (+ scales [PAGES, HKV, PAGE] for fp8)."""
+    shape = k_pages.shape
+    if len(shape) != 4 or v_pages.shape != shape or not k_pages.is_contiguous() or not v_pages.is_contiguous():
+        raise ValueError("pools must be contiguous [PAGES, HKV, PAGE, D] of one shape")
+    fp8 = k_pages.dtype == torch.float8_e4m3fn
+    if v_pages.dtype != k_pages.dtype or not (fp8 or k_pages.dtype == torch.bfloat16):
+        raise TypeError("pools must be float8_e4m3fn or bfloat16")
+    ks = vs = None
+    if fp8:
+        for t in (k_scale, v_scale):
+            if t is None or t.dtype != torch.float32 or t.shape != shape[:3] or not t.is_contiguous():
+                raise ValueError("an fp8 pool needs contiguous float32 k_scale and v_scale [PAGES, HKV, PAGE]")
+        ks, vs = k_scale.data_ptr(), v_scale.data_ptr()
+    return L.Paged(k_pages.data_ptr(), v_pages.data_ptr(), ks, vs, shape[1], shape[3], L.TRB_KV_FP8 if fp8 else L.TRB_KV_BF16, shape[2], shape[0])
+
+
+def _batch(table, lens) -> L.Batch:
+    if table.dtype != torch.int32 or table.dim() != 2 or table.stride(1) != 1:
+        raise ValueError("table must be int32 [B, PAGES] with contiguous rows")
+    if lens.dtype not in (torch.int32, torch.int64) or lens.dim() != 1 or lens.shape[0] != table.shape[0] or not lens.is_contiguous():
+        raise ValueError("lens must be contiguous int32 or int64 [B]")
+    return L.Batch(table.data_ptr(), table.stride(0), lens.data_ptr(), lens.element_size(), table.shape[0], table.shape[1], 0)
+
+
+def paged_append(k, v, k_pages, v_pages, table, lens, k_scale=None, v_scale=None, *, q=None, cu=None, base=0, q_norm_w=None, k_norm_w=None,
+                 eps: float = 1e-6, inv_freq=None, interleaved: bool = False, amplitude: float = 1.0):
+    """Append a step's rows to a paged cache: k, v [T, HKV, D] bf16 (any strides with a contiguous last dim, as views
+    of a fused projection) become own rows lens[b], lens[b] + 1, .. of sequence b; lens [B] int32 / int64 and table [B, PAGES]
+    int32 stay on the device.  cu [B + 1] int32: first row of each sequence; None: T / B rows each.  Slots with lens[b] < 0
+    and rows from cu[B] on are skipped.  On the way k (and q [T, HQ, D], if given) pass the heads' RMSNorm with
+    the (1 + w) gain (where weights are given) and the rotation by (base + row) * inv_freq (float64 [rotary_dim / 2] from
+    `rope.frequencies`; base: an int or a device integer, the length of a shared prefix).  Pairs are (x, x + rotary_dim / 2) or,
+    interleaved, (2x, 2x + 1).  Returns the finished q [T, HQ, D] (None without q).  Two sequences of one call must not
+    share the pages they write."""
+    index = _on_device(k, v, k_pages, v_pages, k_scale, v_scale, table, lens, q, cu, q_norm_w, k_norm_w, inv_freq)
+    pool, batch = _pool(k_pages, v_pages, k_scale, v_scale), _batch(table, lens)
+    t, d = k.shape[0], pool.d
+    if k.dim() != 3 or k.shape[1] != pool.hkv or k.shape[2] != d or v.shape != k.shape:
+        raise ValueError("k and v must be [T, HKV, D] of the pool's heads")
+    for x in (k, v, q):
+        if x is not None and (x.dtype != torch.bfloat16 or x.stride(-1) != 1):
+            raise ValueError("q, k, v must be bfloat16 with a contiguous last dim")
+    for w in (q_norm_w, k_norm_w):
+        if w is not None and (w.dtype != torch.bfloat16 or w.shape != (d,) or not w.is_contiguous()):
+            raise ValueError("norm weights must be bfloat16 [D]")
+    b, rows, rd = batch.n_seqs, 0, 0
+    if cu is None:
+        if t % b:
+            raise ValueError("without cu every sequence has the same number of rows")
+        rows = t // b
+    elif cu.dtype != torch.int32 or cu.shape != (b + 1,) or not cu.is_contiguous():
+        raise ValueError("cu must be int32 [B + 1]")
+    if inv_freq is not None:
+        if inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 or not inv_freq.is_contiguous():
+            raise ValueError("inv_freq must be float64 [rotary_dim / 2]")
+        rd = 2 * inv_freq.shape[0]
+    out = None
+    if q is not None:
+        if q.dim() != 3 or q.shape[0] != t or q.shape[2] != d:
+            raise ValueError("q must be [T, HQ, D]")
+        out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+    if t == 0:
+        return out
+    a = L.PagedAppendArgs(q.data_ptr() if q is not None else None, k.data_ptr(), v.data_ptr(), out.data_ptr() if q is not None else None,
+                          q.stride(0) if q is not None else 0, q.stride(1) if q is not None else 0, k.stride(0), k.stride(1), v.stride(0), v.stride(1),
+                          q_norm_w.data_ptr() if q_norm_w is not None else None, k_norm_w.data_ptr() if k_norm_w is not None else None,
+                          inv_freq.data_ptr() if rd else None, cu.data_ptr() if cu is not None else None, t, rows, q.shape[1] if q is not None else 0,
+                          rd, int(interleaved), eps, amplitude, _cursor(base))
+    L.check(L.lib().trb_paged_append(C.byref(pool), C.byref(batch), C.byref(a), torch._C._cuda_getCurrentRawStream(index)), "trb_paged_append")
+    return out
+
+
+def attn_paged(q, k_pages, v_pages, table, lens, k_scale=None, v_scale=None, *, prefix_table=None, prefix_len=0, gate=None, scale=None, out=None):
+    """Attention of a step's new rows over a paged cache: q [B, M, HQ, D] bf16 (from paged_append; the M rows are already
+    appended, lens is still the length before them).  Row i of sequence b sees the prefix_len rows that all sequences
+    share (pages prefix_table [P] int32; prefix_len: an int or a device integer) and its own rows <= lens[b] + i.  Slots with
+    lens[b] < 0 give zeros.  gate (optional): bf16 [B, M, HQ, D] view, out = bf16(o) * bf16(sigmoid(gate)) as in attn_decode_fused.
+    Returns [B, M, HQ, D].  Lengths are read on the device, so a captured step serves all of them."""
+    index = _on_device(q, k_pages, v_pages, k_scale, v_scale, table, lens, prefix_table, gate, out)
+    pool, batch = _pool(k_pages, v_pages, k_scale, v_scale), _batch(table, lens)
+    shape = q.shape
+    if len(shape) != 4 or shape[0] != batch.n_seqs or shape[3] != pool.d or q.dtype != torch.bfloat16 or not q.is_contiguous():
+        raise ValueError("q must be contiguous bf16 [B, M, HQ, D]")
+    m, hq, pages = shape[1], shape[2], 0
+    if prefix_table is not None:
+        if prefix_table.dtype != torch.int32 or prefix_table.dim() != 1 or not prefix_table.is_contiguous():
+            raise ValueError("prefix_table must be contiguous int32 [P]")
+        pages = prefix_table.shape[0]
+        if not isinstance(prefix_len, torch.Tensor) and not 0 <= prefix_len <= pages * pool.page_size:
+            raise ValueError("prefix_len exceeds the pages of prefix_table")
+    elif isinstance(prefix_len, torch.Tensor) or prefix_len != 0:
+        raise ValueError("a prefix needs its prefix_table")
+    rs = hs = 0
+    if gate is not None:
+        if gate.shape != shape or gate.dtype != torch.bfloat16 or gate.stride(3) != 1 or gate.stride(0) != m * gate.stride(1):
+            raise ValueError("gate must be a bf16 [B, M, HQ, D] view with equally spaced rows")
+        rs, hs = gate.stride(1), gate.stride(2)
+    if out is None:
+        out = torch.empty(shape, device=q.device, dtype=q.dtype)
+    elif out.shape != shape or out.dtype != torch.bfloat16 or not out.is_contiguous():
+        raise ValueError("out must be contiguous bf16 [B, M, HQ, D]")
+    lib = L.lib()
+    n = lib.trb_attn_paged_workspace_bytes(C.byref(pool), batch.n_seqs, m, hq, pages)
+    if n == 0:
+        raise ValueError(f"unsupported geometry B={batch.n_seqs} m={m} hq={hq} hkv={pool.hkv} d={pool.d} page={pool.page_size}")
+    # a fresh buffer for every call: calls on other streams and in other captured graphs never share one
+    ws = torch.empty(n, device=q.device, dtype=torch.uint8)
+    a = L.AttnPagedArgs(q.data_ptr(), out.data_ptr(), gate.data_ptr() if gate is not None else None, rs, hs, m, hq,
+                        pool.d ** -0.5 if scale is None else scale, pages, prefix_table.data_ptr() if pages else None, _cursor(prefix_len),
+                        ws.data_ptr(), n)
+    L.check(lib.trb_attn_paged(C.byref(pool), C.byref(batch), C.byref(a), torch._C._cuda_getCurrentRawStream(index)), "trb_attn_paged")
+    return out
+
+
+_PROB_TYPES = {torch.float32: L.TRB_DT_F32, torch.bfloat16: L.TRB_DT_BF16, torch.float16: L.TRB_DT_F16}
+
+
+def spec_verify(probs, drafts, u, *, draft_probs=None, n_drafts=None, lens=None):
+    """Verify K drafted tokens of every sequence by sampling (spec_commit is the greedy form): probs [B, K + 1, V] are the
+    target's probabilities (fp32, bf16 or fp16, last dim contiguous), drafts [B, K] int64, u [B, K + 1] fp32 numbers in [0, 1),
+    draft_probs [B, K, V] in the type of probs (None: the drafts were certain).  Draft i stands while u[b, i] * q < p; the next
+    token is drawn with u[b, K] from the first fallen draft's residual, or from the row behind the last draft.
+    n_drafts [B] int32 (optional): drafts of each sequence, negative for an empty slot.  lens [B] (optional) is
+    advanced by what was accepted plus one.  Returns tokens [B, K + 1] int64 (accepted drafts, the new token, then -1) and
+    n_accepted [B] int64, both on the device."""
+    index = _on_device(probs, drafts, u, draft_probs, n_drafts, lens)
+    if probs.dim() != 3 or probs.dtype not in _PROB_TYPES or probs.stride(2) != 1:
+        raise ValueError("probs must be fp32, bf16 or fp16 [B, K + 1, V] with a contiguous last dim")
+    b, k, vocab = probs.shape[0], probs.shape[1] - 1, probs.shape[2]
+    if k < 0 or drafts.shape != (b, k) or drafts.dtype != torch.int64 or not drafts.is_contiguous():
+        raise ValueError("drafts must be contiguous int64 [B, K]")
+    if u.shape != (b, k + 1) or u.dtype != torch.float32 or not u.is_contiguous():
+        raise ValueError("u must be contiguous float32 [B, K + 1]")
+    qs = (0, 0)
+    if draft_probs is not None:
+        if draft_probs.shape != (b, k, vocab) or draft_probs.dtype != probs.dtype or draft_probs.stride(2) != 1:
+            raise ValueError("draft_probs must be [B, K, V] of the type of probs with a contiguous last dim")
+        qs = draft_probs.stride()
+    if n_drafts is not None and (n_drafts.shape != (b,) or n_drafts.dtype != torch.int32 or not n_drafts.is_contiguous()):
+        raise ValueError("n_drafts must be contiguous int32 [B]")
+    if lens is not None and (lens.shape != (b,) or lens.dtype not in (torch.int32, torch.int64) or not lens.is_contiguous()):
+        raise ValueError("lens must be contiguous int32 or int64 [B]")
+    tokens = torch.empty(b, k + 1, device=probs.device, dtype=torch.int64)
+    n = torch.empty(b, device=probs.device, dtype=torch.int64)
+    if b == 0:
+        return tokens, n
+    a = L.SpecVerifyArgs(probs.data_ptr(), draft_probs.data_ptr() if draft_probs is not None else None, probs.stride(0), probs.stride(1), qs[0], qs[1],
+                         drafts.data_ptr(), u.data_ptr(), n_drafts.data_ptr() if n_drafts is not None else None, tokens.data_ptr(), n.data_ptr(),
+                         lens.data_ptr() if lens is not None else None, lens.element_size() if lens is not None else 0, b, k, vocab,
+                         _PROB_TYPES[probs.dtype], 0)
+    L.check(L.lib().trb_spec_verify(C.byref(a), torch._C._cuda_getCurrentRawStream(index)), "trb_spec_verify")
+    return tokens, n
