@@ -53,4 +53,25 @@ __device__ __forceinline__ long long load_len(const BatchView &b, int i) {
     return b.lens_width == 4 ? (long long)((const int *)b.lens)[i] : ((const long long *)b.lens)[i];
 }
 
+// Rows of the prefix, and rows of one sequence's own pages, that this step may see (clamped to what the tables hold).
+__device__ __forceinline__ int paged_prefix_rows(const Cursor &len, int pages, int page_shift, bool report) {
+    long long n = pages > 0 ? load_cursor(len) : 0;
+    const long long most = (long long)pages << page_shift;
+    if (n < 0 || n > most) {
+        if (report) raise_status(TRB_ST_CURSOR_RANGE);
+        n = n < 0 ? 0 : most;
+    }
+    return (int)n;
+}
+__device__ __forceinline__ int paged_own_rows(const BatchView &b, int seq, int m, int page_shift, bool report) {
+    const long long len = load_len(b, seq);
+    if (len < 0) return -1;                                            // an empty slot
+    const long long most = (long long)b.table_pages << page_shift;
+    if (len + m > most) {
+        if (report) raise_status(TRB_ST_CURSOR_RANGE);
+        return (int)most;
+    }
+    return (int)(len + m);
+}
+
 }  // namespace trb

@@ -16,6 +16,7 @@
 // conflicts) instead of fragments, and the chunk's order is carried by how Q is laid out and O is read back.  e4m3 codes become f16 in
 // registers; the K scale multiplies the score, the V scale moves into the exponent, so codes are never scaled.
 #include "paged.cuh"
+#include "paged_prefix.cuh"
 
 namespace trb {
 
@@ -33,6 +34,9 @@ struct PagedAttnParams {
     const int *prefix_table;
     int prefix_pages;                  // rows of the prefix that the scan itself reads come from here (0: none)
     Cursor prefix_len;
+    int after_prefix;                  // launched behind paged_prefix_kernel, which reads the prefix
+    int splits;                        // its pieces (0: none)
+    const float *px_ml, *px_acc;       // [splits][hkv][n_seqs * m * g][2] and [..][D]
     int ctas;                          // CTAs per (kv head, row group)
     int groups;                        // groups of 8 * NS query rows
     int *plan;                         // [n_seqs][2]: first and last CTA with keys of the sequence
@@ -49,27 +53,6 @@ __device__ __forceinline__ uint4 ld_shared_v4(uint32_t a) {
     uint4 v;
     asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
     return v;
-}
-
-// Rows of the prefix, and rows of one sequence's own pages, that this step may see (clamped to what the tables hold).
-__device__ __forceinline__ int paged_prefix_rows(const Cursor &len, int pages, int page_shift, bool report) {
-    long long n = pages > 0 ? load_cursor(len) : 0;
-    const long long most = (long long)pages << page_shift;
-    if (n < 0 || n > most) {
-        if (report) raise_status(TRB_ST_CURSOR_RANGE);
-        n = n < 0 ? 0 : most;
-    }
-    return (int)n;
-}
-__device__ __forceinline__ int paged_own_rows(const BatchView &b, int seq, int m, int page_shift, bool report) {
-    const long long len = load_len(b, seq);
-    if (len < 0) return -1;                                            // an empty slot
-    const long long most = (long long)b.table_pages << page_shift;
-    if (len + m > most) {
-        if (report) raise_status(TRB_ST_CURSOR_RANGE);
-        return (int)most;
-    }
-    return (int)(len + m);
 }
 
 template <int D_, bool FP8_, int NS_> struct ScanCfg {
@@ -102,7 +85,9 @@ __global__ void __launch_bounds__(PS_THREADS) paged_scan_kernel(const PagedAttnP
     const int j = blockIdx.y % p.c.hkv, grp = blockIdx.y / p.c.hkv, hg = blockIdx.y;
     const int rows = p.g * p.m, r0 = grp * 8 * NS;
     const uint32_t ring = smem_u32(ps_smem + warp * C::RING);
-    pdl_wait();
+    // behind the prefix kernel this one starts when that has passed its own wait: everything before both is complete, and what
+    // the two write is apart.  It then waits at its end, so that its completion says the same of the prefix kernel.
+    if (!p.after_prefix) pdl_wait();
     pdl_launch_dependents();
 
     // ---- the line of pipeline steps: sm_cnt[b] = steps before sequence b
@@ -141,9 +126,9 @@ __global__ void __launch_bounds__(PS_THREADS) paged_scan_kernel(const PagedAttnP
             p.plan[2 * b + 1] = hi > lo ? (int)(((long long)hi * active - 1) / total) : -1;       // ... and step hi - 1
         }
     }
-    if ((int)blockIdx.x >= active || total == 0) return;
+    if ((int)blockIdx.x >= active || total == 0) { pdl_wait(); return; }
     const int lo = (int)((long long)blockIdx.x * total / active), hi = (int)(((long long)blockIdx.x + 1) * total / active);
-    if (lo >= hi) return;
+    if (lo >= hi) { pdl_wait(); return; }
     int seq;
     {
         int a = 0, z = p.b.n_seqs;                                      // last sequence that starts at or before lo
@@ -493,9 +478,10 @@ __global__ void __launch_bounds__(PS_THREADS) paged_scan_kernel(const PagedAttnP
         }
         __syncthreads();
     }
+    pdl_wait();
 }
 
-// Joins the partials of a query row, one warp per row: at most plan[1] - plan[0] + 1 pieces of the scan.  The weights
+// Joins the partials of a query row, one warp per row: plan[1] - plan[0] + 1 pieces of the scan, then those of the prefix.  The weights
 // exp2(m - max) are found 32 pieces at a time, one per lane.  Latency-bound: a few KB per row, all from L2.
 template <int D>
 __global__ void __launch_bounds__(256) paged_merge_kernel(const PagedAttnParams p, const int ns) {
@@ -508,32 +494,39 @@ __global__ void __launch_bounds__(256) paged_merge_kernel(const PagedAttnParams 
     const int h = (int)(row % p.hq), i = (int)(row / p.hq % p.m), seq = (int)(row / p.hq / p.m);
     const int j = h / p.g, r = i * p.g + h % p.g, grp = r / (8 * ns), col = r % (8 * ns);
     const int c0 = p.plan[2 * seq], c1 = p.plan[2 * seq + 1];
-    const long long slot0 = (long long)(grp * p.c.hkv + j) * (p.ctas + p.b.n_seqs) + seq;
+    const long long slot0 = ((long long)(grp * p.c.hkv + j) * (p.ctas + p.b.n_seqs) + seq) * 8 * ns + col;
+    const long long px0 = ((long long)j * p.b.n_seqs + seq) * p.g * p.m + r, px_step = (long long)p.c.hkv * p.b.n_seqs * p.g * p.m;
     float mx = -INFINITY, l = 0.f, o[EPT];
 #pragma unroll
     for (int e = 0; e < EPT; ++e) o[e] = 0.f;
-    for (int base = c0; base <= c1; base += 32) {
-        const int n = min(32, c1 - base + 1);
-        float2 ml = make_float2(-INFINITY, 0.f);
-        if (lane < n) ml = *reinterpret_cast<const float2 *>(p.part_ml + ((slot0 + base + lane) * 8 * ns + col) * 2);
-        const float m_new = fmaxf(mx, warp_max(ml.x));
-        const float w = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - m_new);
-        const float alpha = mx == -INFINITY ? 0.f : fast_exp2(mx - m_new);
-        l = l * alpha + warp_sum(w == 0.f && ml.y == ml.y ? 0.f : ml.y * w);
+    // pieces at part row + x * step, x in [x0, x1]
+    auto join = [&](const float *part_ml, const float *part_acc, long long at, long long step, int x0, int x1) {
+        for (int base = x0; base <= x1; base += 32) {
+            const int n = min(32, x1 - base + 1);
+            float2 ml = make_float2(-INFINITY, 0.f);
+            if (lane < n) ml = *reinterpret_cast<const float2 *>(part_ml + (at + (base + lane) * step) * 2);
+            const float m_new = fmaxf(mx, warp_max(ml.x));
+            const float w = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - m_new);
+            const float alpha = mx == -INFINITY ? 0.f : fast_exp2(mx - m_new);
+            l = l * alpha + warp_sum(ml.y * w);
 #pragma unroll
-        for (int e = 0; e < EPT; ++e) o[e] *= alpha;
-        mx = m_new;
-        for (int x = 0; x < n; ++x) {
-            const float wx = __shfl_sync(0xffffffffu, w, x);
-            const float4 *src = reinterpret_cast<const float4 *>(p.part_acc + ((slot0 + base + x) * 8 * ns + col) * D + lane * EPT);
+            for (int e = 0; e < EPT; ++e) o[e] *= alpha;
+            mx = m_new;
+            for (int x = 0; x < n; ++x) {
+                const float wx = __shfl_sync(0xffffffffu, w, x);
+                if (__shfl_sync(0xffffffffu, ml.y, x) == 0.f) continue;        // a piece without keys (its acc is not written)
+                const float4 *src = reinterpret_cast<const float4 *>(part_acc + (at + (base + x) * step) * D + lane * EPT);
 #pragma unroll
-            for (int e = 0; e < EPT / 4; ++e) {
-                const float4 v = src[e];
-                o[e * 4] = fmaf(v.x, wx, o[e * 4]); o[e * 4 + 1] = fmaf(v.y, wx, o[e * 4 + 1]);
-                o[e * 4 + 2] = fmaf(v.z, wx, o[e * 4 + 2]); o[e * 4 + 3] = fmaf(v.w, wx, o[e * 4 + 3]);
+                for (int e = 0; e < EPT / 4; ++e) {
+                    const float4 v = src[e];
+                    o[e * 4] = fmaf(v.x, wx, o[e * 4]); o[e * 4 + 1] = fmaf(v.y, wx, o[e * 4 + 1]);
+                    o[e * 4 + 2] = fmaf(v.z, wx, o[e * 4 + 2]); o[e * 4 + 3] = fmaf(v.w, wx, o[e * 4 + 3]);
+                }
             }
         }
-    }
+    };
+    join(p.part_ml, p.part_acc, slot0, 8 * ns, c0, c1);
+    if (p.splits > 0 && load_len(p.b, seq) >= 0) join(p.px_ml, p.px_acc, px0, px_step, 0, p.splits - 1);
     const float inv = l == 0.f ? 0.f : __fdiv_rn(1.f, l);                 // a row that sees no key is zero
     __nv_bfloat16 ob[EPT];
 #pragma unroll
@@ -551,23 +544,58 @@ __global__ void __launch_bounds__(256) paged_merge_kernel(const PagedAttnParams 
     else *reinterpret_cast<uint2 *>(dst) = *reinterpret_cast<const uint2 *>(ob);
 }
 
-// How a call is cut: query-row slices per CTA, row groups, CTAs per (kv head, group), and where its partials lie.
+// How a call is cut: query-row slices per CTA, row groups, CTAs per (kv head, group), pieces of the prefix and blocks of 128 query
+// rows of its kernel (0: the scan reads the prefix itself), and where the partials lie.
 struct PagedAttnPlan {
-    int ns, groups, ctas;
-    size_t off_ml, off_acc, bytes;
+    int ns, groups, ctas, splits, blocks;
+    size_t off_ml, off_acc, off_px_ml, off_px_acc, bytes;
 };
-static PagedAttnPlan paged_attn_plan(int d, bool fp8, int hkv, int hq, int n_seqs, int m) {
+static PagedAttnPlan paged_attn_plan(int d, bool fp8, int hkv, int hq, int n_seqs, int m, long long prefix_rows) {
     PagedAttnPlan o;
     const int rows = hq / hkv * m;
     o.ns = rows <= 8 ? 1 : 2;
     o.groups = (rows + 8 * o.ns - 1) / (8 * o.ns);
     const int per_sm = fp8 ? 2 : 1;                                       // CTAs that fit an SM (shared memory)
     o.ctas = std::max(1, sm_count() * per_sm / (hkv * o.groups));
-    const size_t slots = (size_t)hkv * o.groups * (o.ctas + n_seqs) * 8 * o.ns;
-    o.off_ml = ((size_t)n_seqs * 8 + 255) / 256 * 256;
-    o.off_acc = (o.off_ml + slots * 8 + 255) / 256 * 256;
-    o.bytes = o.off_acc + slots * d * 4;
+    o.splits = o.blocks = 0;
+    if (prefix_rows > 0 && n_seqs > 1) {
+        const int tile = fp8 || d == 128 ? 128 : 64;
+        const long long tiles = (prefix_rows + tile - 1) / tile;
+        o.blocks = (int)(((long long)n_seqs * rows + 127) / 128);
+        const int units = o.blocks * hkv;
+        // one wave of CTAs, and at least two tiles for each
+        o.splits = (int)std::max(1LL, std::min((long long)sm_count() / units, tiles / 2));
+    }
+    auto up = [](size_t x) { return (x + 255) / 256 * 256; };
+    const size_t slots = (size_t)hkv * o.groups * (o.ctas + n_seqs) * 8 * o.ns, px = (size_t)o.splits * hkv * n_seqs * rows;
+    o.off_ml = up((size_t)n_seqs * 8);
+    o.off_acc = up(o.off_ml + slots * 8);
+    o.off_px_ml = up(o.off_acc + slots * d * 4);
+    o.off_px_acc = up(o.off_px_ml + px * 8);
+    o.bytes = up(o.off_px_acc + px * d * 4);
     return o;
+}
+
+template <typename C>
+static int launch_prefix(const PagedAttnParams &p, const PagedAttnPlan &plan, cudaStream_t st) {
+    static bool attr_set[64] = {};
+    int dev = 0, rc;
+    TRB_CUDA_CHECK(cudaGetDevice(&dev));
+    if (!attr_set[dev & 63]) {
+        TRB_CUDA_CHECK(cudaFuncSetAttribute(paged_prefix_kernel<C>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
+        attr_set[dev & 63] = true;
+    }
+    PrefixParams x;
+    x.c = p.c; x.q = p.q; x.n_seqs = p.b.n_seqs; x.m = p.m; x.hq = p.hq; x.g = p.g; x.scale_log2 = p.scale_log2;
+    x.table = p.prefix_table; x.pages = p.prefix_pages; x.len = p.prefix_len;
+    x.splits = plan.splits; x.blocks = plan.blocks; x.part_ml = const_cast<float *>(p.px_ml); x.part_acc = const_cast<float *>(p.px_acc);
+    // the pool as [num_pages * hkv][page_size] rows; a box is a page, or a tile of a larger page
+    CUtensorMap mk, mv;
+    const int page = 1 << p.c.page_shift, box = std::min(page, (int)C::BN);
+    if ((rc = get_row_tile_map(p.c.k, page, (int)(p.c.num_pages * p.c.hkv), C::ROWB, box, &mk))) return rc;
+    if ((rc = get_row_tile_map(p.c.v, page, (int)(p.c.num_pages * p.c.hkv), C::ROWB, box, &mv))) return rc;
+    TRB_CUDA_CHECK(launch_kernel(paged_prefix_kernel<C>, dim3((unsigned)plan.splits * plan.blocks * p.c.hkv), dim3(PX_THREADS), C::SMEM, st, true, mk, mv, x));
+    return TRB_OK;
 }
 
 template <typename C>
@@ -596,7 +624,7 @@ static int check_paged_geometry(const trb_paged_t *pool, int n_seqs, int m, int 
 extern "C" size_t trb_attn_paged_workspace_bytes(const trb_paged_t *pool, int32_t n_seqs, int32_t m, int32_t hq, int32_t prefix_pages) {
     PagedView v;
     if (make_paged_view(pool, &v) || check_paged_geometry(pool, n_seqs, m, hq, prefix_pages)) return 0;
-    return paged_attn_plan(pool->d, v.ks != nullptr, pool->hkv, hq, n_seqs, m).bytes;
+    return paged_attn_plan(pool->d, v.ks != nullptr, pool->hkv, hq, n_seqs, m, (long long)prefix_pages << v.page_shift).bytes;
 }
 
 extern "C" int trb_attn_paged(const trb_paged_t *pool, const trb_batch_t *batch, const trb_attn_paged_args_t *a, trb_stream_t stream) {
@@ -611,7 +639,7 @@ extern "C" int trb_attn_paged(const trb_paged_t *pool, const trb_batch_t *batch,
     if (((((long long)a->prefix_pages + batch->table_pages) << p.c.page_shift) / 16 + 2) * batch->n_seqs > 0x7fffffffLL) return TRB_E_UNSUPPORTED;
     if ((((uintptr_t)a->q | (uintptr_t)a->out) & 15) || ((uintptr_t)a->workspace & 255) || ((uintptr_t)a->prefix_table & 3) || ((uintptr_t)a->gate & 1)) return TRB_E_ALIGN;
     const bool fp8 = p.c.ks != nullptr;
-    const PagedAttnPlan plan = paged_attn_plan(pool->d, fp8, pool->hkv, a->hq, batch->n_seqs, a->m);
+    const PagedAttnPlan plan = paged_attn_plan(pool->d, fp8, pool->hkv, a->hq, batch->n_seqs, a->m, (long long)a->prefix_pages << p.c.page_shift);
     if (a->workspace_bytes < plan.bytes) return TRB_E_CAPACITY;
     p.q = (const __nv_bfloat16 *)a->q; p.out = (__nv_bfloat16 *)a->out; p.gate = (const __nv_bfloat16 *)a->gate;
     p.gate_rs = a->gate_row_stride; p.gate_hs = a->gate_head_stride;
@@ -620,8 +648,16 @@ extern "C" int trb_attn_paged(const trb_paged_t *pool, const trb_batch_t *batch,
     p.ctas = plan.ctas; p.groups = plan.groups;
     uint8_t *ws = (uint8_t *)a->workspace;
     p.plan = (int *)ws; p.part_ml = (float *)(ws + plan.off_ml); p.part_acc = (float *)(ws + plan.off_acc);
+    p.px_ml = (const float *)(ws + plan.off_px_ml); p.px_acc = (const float *)(ws + plan.off_px_acc);
+    p.splits = plan.splits; p.after_prefix = plan.splits > 0;
     cudaStream_t st = (cudaStream_t)stream;
     pdl_forget(st);
+    if (plan.splits > 0) {
+        rc = pool->d == 256 ? (fp8 ? launch_prefix<PrefixCfg<256, true>>(p, plan, st) : launch_prefix<PrefixCfg<256, false>>(p, plan, st))
+                            : (fp8 ? launch_prefix<PrefixCfg<128, true>>(p, plan, st) : launch_prefix<PrefixCfg<128, false>>(p, plan, st));
+        if (rc) return rc;
+        p.prefix_pages = 0;                                               // the scan has the own rows alone
+    }
     if (plan.ns == 1) rc = pool->d == 256 ? (fp8 ? launch_scan<ScanCfg<256, true, 1>>(p, st) : launch_scan<ScanCfg<256, false, 1>>(p, st))
                                           : (fp8 ? launch_scan<ScanCfg<128, true, 1>>(p, st) : launch_scan<ScanCfg<128, false, 1>>(p, st));
     else rc = pool->d == 256 ? (fp8 ? launch_scan<ScanCfg<256, true, 2>>(p, st) : launch_scan<ScanCfg<256, false, 2>>(p, st))
