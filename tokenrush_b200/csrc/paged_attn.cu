@@ -65,11 +65,12 @@ template <int D_, bool FP8_, int NS_> struct ScanCfg {
     static constexpr int KJ = CPR / 4, VC = CPR / 8;                   // chunks per lane of a K row, of a V row
     static constexpr int KS = D / 16;                                  // MMA steps of a QK product = row tiles of a PV product
     static constexpr int OFF_Q = PS_WARPS * RING;                      // [NS][KS][32] uint2
-    static constexpr int OFF_QINV = OFF_Q + NS * KS * 256;             // [8 NS] floats
-    static constexpr int OFF_ML = OFF_QINV + NS * 32;                  // [warps][8 NS][2] floats
+    static constexpr int OFF_QINV = OFF_Q + (NS > 1 ? NS * KS * 256 : 0);      // [warps or slices][8] floats
+    static constexpr int OFF_ML = OFF_QINV + PS_WARPS * 32;                  // [warps][8 NS][2] floats
     static constexpr int OFF_CNT = OFF_ML + PS_WARPS * NS * 64;        // [PG_MAX_SEQS + 1] ints, then 8 for the scan
     static constexpr int SMEM = OFF_CNT + (PG_MAX_SEQS + 16) * 4;
-    static_assert(NS * 8 * D * 4 <= RING, "a warp's accumulators are exchanged through its ring");
+    static constexpr int RED = (NS * 8 * D * 4 + STAGE + SC - 1) / (STAGE + SC);   // stages that a warp's accumulators take when they are exchanged
+    static_assert(RED < PS_STAGES && NS <= PS_WARPS, "the exchange leaves a stage for the next sequence");
 };
 
 template <typename C>
@@ -137,105 +138,128 @@ __global__ void __launch_bounds__(PS_THREADS) paged_scan_kernel(const PagedAttnP
         while (sm_cnt[seq + 1] <= lo) ++seq;                            // (skips slots without steps that start at lo)
     }
 
-    for (; seq < p.b.n_seqs && sm_cnt[seq] < hi; ++seq) {
-        const int s0 = max(lo, sm_cnt[seq]) - sm_cnt[seq], s1 = min(hi, sm_cnt[seq + 1]) - sm_cnt[seq];
-        if (s1 <= s0) continue;
-        const int own = paged_own_rows(p.b, seq, p.m, p.c.page_shift, false);
-        const long long len = load_len(p.b, seq);
-        const int *own_table = p.b.table + seq * p.b.table_stride;
-
-        // ---- pipeline of this warp: steps s0 + warp, s0 + warp + 4, ..
-        auto page_of = [&](int tile) -> int {                          // pool page of a tile, -1: none
-            const int x = tile - prefix_tiles;
-            int pg = -1;
-            if (x < 0) pg = p.prefix_table[(tile * 16) >> p.c.page_shift];
-            else if (x * 16 < own) pg = own_table[(x * 16) >> p.c.page_shift];
-            else return -1;
-            if (pg < 0 || pg >= p.c.num_pages) { if (lane == 0) raise_status(TRB_ST_CURSOR_RANGE); pg = -1; }
-            return pg;
-        };
-        auto load_step = [&](int step, int stage, const int (&pages)[SUB]) {
-            const uint32_t base = ring + stage * (C::STAGE + C::SC);
+    // ---- pipeline of a warp over the steps s0 + warp, s0 + warp + 4, .. of the current sequence
+    int s0, s1, own, steps, pages[SUB];
+    long long len;
+    const int *own_table;
+    auto page_of = [&](int tile) -> int {                              // pool page of a tile, -1: none
+        const int x = tile - prefix_tiles;
+        int pg = -1;
+        if (x < 0) pg = p.prefix_table[(tile * 16) >> p.c.page_shift];
+        else if (x * 16 < own) pg = own_table[(x * 16) >> p.c.page_shift];
+        else return -1;
+        if (pg < 0 || pg >= p.c.num_pages) { if (lane == 0) raise_status(TRB_ST_CURSOR_RANGE); pg = -1; }
+        return pg;
+    };
+    auto fetch_pages = [&](int k) {
 #pragma unroll
-            for (int sb = 0; sb < SUB; ++sb) {
-                const int tile = step * SUB + sb, x = tile - prefix_tiles;
-                const int row = x < 0 ? tile * 16 : x * 16, limit = pages[sb] < 0 ? 0 : (x < 0 ? n_prefix : own);
-                const int left = limit - row;                          // rows of the tile that exist; the others are zero
-                const long long first = pages[sb] < 0 ? 0
-                                        : ((((long long)pages[sb] * p.c.hkv + j) << p.c.page_shift) + (row & ((1 << p.c.page_shift) - 1)));
-                const uint8_t *ks = p.c.k + first * C::ROWB + lane * 16, *vs = p.c.v + first * C::ROWB + lane * 16;
-                const uint32_t kd = base + sb * 2 * C::TILE, vd = kd + C::TILE;
+        for (int sb = 0; sb < SUB; ++sb) pages[sb] = k < steps ? page_of((s0 + warp + k * PS_WARPS) * SUB + sb) : -1;
+    };
+    auto load_step = [&](int step, int stage, const int (&pg)[SUB]) {
+        const uint32_t base = ring + stage * (C::STAGE + C::SC);
 #pragma unroll
-                for (int i = 0; i < CPR / 2; ++i) {                    // 16 rows x CPR chunks over 32 lanes
-                    const int idx = i * 32 + lane, r = idx / CPR, ch = idx % CPR;
-                    const uint32_t n = r < left ? 16u : 0u;
-                    const uint32_t off = r < left ? i * 512 : 0;
-                    cp_async_16(kd + r * C::ROWB + ((ch ^ ((r & 1) << 2)) << 4), ks + off, n);
-                    cp_async_16(vd + r * C::ROWB + ((ch ^ (r & 6)) << 4), vs + off, n);
-                }
-                if constexpr (FP8) {
-                    const bool ok = (lane & 15) < left;
-                    const float *sc = (lane < 16 ? p.c.ks : p.c.vs) + first + (ok ? (lane & 15) : 0);
-                    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(base + C::STAGE + sb * 128 + lane * 4), "l"(sc), "r"(ok ? 4u : 0u) : "memory");
-                }
+        for (int sb = 0; sb < SUB; ++sb) {
+            const int tile = step * SUB + sb, x = tile - prefix_tiles;
+            const int row = x < 0 ? tile * 16 : x * 16, limit = pg[sb] < 0 ? 0 : (x < 0 ? n_prefix : own);
+            const int left = limit - row;                              // rows of the tile that exist; the others are zero
+            const long long first = pg[sb] < 0 ? 0 : ((((long long)pg[sb] * p.c.hkv + j) << p.c.page_shift) + (row & ((1 << p.c.page_shift) - 1)));
+            const uint8_t *ks = p.c.k + first * C::ROWB + lane * 16, *vs = p.c.v + first * C::ROWB + lane * 16;
+            const uint32_t kd = base + sb * 2 * C::TILE, vd = kd + C::TILE;
+#pragma unroll
+            for (int i = 0; i < CPR / 2; ++i) {                        // 16 rows x CPR chunks over 32 lanes
+                const int idx = i * 32 + lane, r = idx / CPR, ch = idx % CPR;
+                const uint32_t n = r < left ? 16u : 0u;
+                const uint32_t off = r < left ? i * 512 : 0;
+                cp_async_16(kd + r * C::ROWB + ((ch ^ ((r & 1) << 2)) << 4), ks + off, n);
+                cp_async_16(vd + r * C::ROWB + ((ch ^ (r & 6)) << 4), vs + off, n);
             }
-            cp_async_commit();
-        };
-        const int steps = s1 - s0 > warp ? (s1 - s0 - warp + PS_WARPS - 1) / PS_WARPS : 0;
-        int pages[SUB];
-        auto fetch_pages = [&](int k) {
+            if constexpr (FP8) {
+                const bool ok = (lane & 15) < left;
+                const float *sc = (lane < 16 ? p.c.ks : p.c.vs) + first + (ok ? (lane & 15) : 0);
+                asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(base + C::STAGE + sb * 128 + lane * 4), "l"(sc), "r"(ok ? 4u : 0u) : "memory");
+            }
+        }
+        cp_async_commit();
+    };
+    // step k of a sequence goes to stage (k + RED) mod PS_STAGES: the first RED stages hold the accumulators that the warps
+    // exchange at the end of the sequence before, while the first steps of this one are already on their way
+    constexpr int RED = C::RED, EARLY = PS_STAGES - RED;
+    auto request = [&](int k) {
+        int now[SUB];
 #pragma unroll
-            for (int sb = 0; sb < SUB; ++sb) pages[sb] = k < steps ? page_of((s0 + warp + k * PS_WARPS) * SUB + sb) : -1;
-        };
+        for (int sb = 0; sb < SUB; ++sb) now[sb] = pages[sb];
+        fetch_pages(k + 1);
+        if (k < steps) load_step(s0 + warp + k * PS_WARPS, (k + RED) % PS_STAGES, now);
+        else cp_async_commit();
+    };
+    auto begin = [&]() {                                               // sequence seq: its piece, and the first EARLY steps
+        s0 = max(lo, sm_cnt[seq]) - sm_cnt[seq];
+        s1 = min(hi, sm_cnt[seq + 1]) - sm_cnt[seq];
+        own = paged_own_rows(p.b, seq, p.m, p.c.page_shift, false);
+        len = load_len(p.b, seq);
+        own_table = p.b.table + seq * p.b.table_stride;
+        steps = s1 - s0 > warp ? (s1 - s0 - warp + PS_WARPS - 1) / PS_WARPS : 0;
         fetch_pages(0);
 #pragma unroll
-        for (int k = 0; k < PS_STAGES - 1; ++k) {
-            int now[SUB];
+        for (int k = 0; k < (EARLY < PS_STAGES - 1 ? EARLY : PS_STAGES - 1); ++k) request(k);
+    };
+    begin();
+    while (true) {
+        const int now = seq;
 #pragma unroll
-            for (int sb = 0; sb < SUB; ++sb) now[sb] = pages[sb];
-            fetch_pages(k + 1);
-            if (k < steps) load_step(s0 + warp + k * PS_WARPS, k, now);
-            else cp_async_commit();
-        }
+        for (int k = EARLY; k < PS_STAGES - 1; ++k) request(k);
 
         // ---- the query rows as MMA fragments: step (jj, w) of lane (g, t) holds dims of chunk 4 jj + t.  e4m3: f16 with a power-of-two
         // factor for each row (a bf16 value may lie outside f16's range); bf16: as they are.
-        for (int s = warp; s < NS; s += PS_WARPS) {
+        constexpr int DPC = FP8 ? 16 : 8;                               // dims of a chunk
+        uint2 qf[KS];
+        float q_inv = 1.f;                                             // of row g of the slice
+        auto load_q = [&](int s) {
             const int r = r0 + s * 8 + g;
             const bool ok = r < rows;
-            const __nv_bfloat16 *src = p.q + (((long long)seq * p.m + (ok ? r / p.g : 0)) * p.hq + j * p.g + (ok ? r % p.g : 0)) * D;
-            constexpr int DPC = FP8 ? 16 : 8;                           // dims of a chunk
-            float mult = 1.f;
+            const __nv_bfloat16 *src = p.q + (((long long)now * p.m + (ok ? r / p.g : 0)) * p.hq + j * p.g + (ok ? r % p.g : 0)) * D;
+#pragma unroll
+            for (int jj = 0; jj < KJ; ++jj)
+#pragma unroll
+                for (int x = 0; x < DPC / 8; ++x) {
+                    const uint4 v = *reinterpret_cast<const uint4 *>(src + (4 * jj + t) * DPC + x * 8);
+                    qf[jj * (DPC / 4) + 2 * x] = ok ? make_uint2(v.x, v.y) : make_uint2(0u, 0u);
+                    qf[jj * (DPC / 4) + 2 * x + 1] = ok ? make_uint2(v.z, v.w) : make_uint2(0u, 0u);
+                }
             if constexpr (FP8) {
                 float amax = 0.f;
-                for (int jj = 0; jj < KJ; ++jj)
 #pragma unroll
-                    for (int x = 0; x < DPC; ++x) amax = fmaxf(amax, fabsf(__bfloat162float(src[(4 * jj + t) * DPC + x])));
+                for (int x = 0; x < KS; ++x) {
+                    const float2 a = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&qf[x].x));
+                    const float2 b = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&qf[x].y));
+                    amax = fmaxf(amax, fmaxf(fmaxf(fabsf(a.x), fabsf(a.y)), fmaxf(fabsf(b.x), fabsf(b.y))));
+                }
                 amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
                 amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
                 int e = (int)((__float_as_uint(amax) >> 23) & 0xffu) - 127;
                 e = amax == 0.f ? 0 : max(-90, min(90, e));
-                mult = __uint_as_float((uint32_t)(127 - e) << 23);
-                if (t == 0) sm_qinv[s * 8 + g] = __uint_as_float((uint32_t)(127 + e) << 23);
-            }
-            for (int jj = 0; jj < KJ; ++jj)
+                const float mult = __uint_as_float((uint32_t)(127 - e) << 23);
+                q_inv = __uint_as_float((uint32_t)(127 + e) << 23);
 #pragma unroll
-                for (int x = 0; x < DPC / 4; ++x) {
-                    const uint2 raw = *reinterpret_cast<const uint2 *>(src + (4 * jj + t) * DPC + x * 4);
-                    uint2 w = ok ? raw : make_uint2(0u, 0u);
-                    if constexpr (FP8) {
-                        const float2 a = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&w.x));
-                        const float2 b = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&w.y));
-                        w = make_uint2(pack_f16x2(a.x * mult, a.y * mult), pack_f16x2(b.x * mult, b.y * mult));
-                    }
-                    sm_q[(s * KS + jj * (DPC / 4) + x) * 32 + lane] = w;
+                for (int x = 0; x < KS; ++x) {
+                    const float2 a = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&qf[x].x));
+                    const float2 b = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&qf[x].y));
+                    qf[x] = make_uint2(pack_f16x2(a.x * mult, a.y * mult), pack_f16x2(b.x * mult, b.y * mult));
                 }
-        }
-        __syncthreads();
-        uint2 qf[NS == 1 ? KS : 1];
+            }
+        };
         if constexpr (NS == 1) {
+            load_q(0);                                                 // every warp for itself, in registers
+            if (t == 0) sm_qinv[warp * 8 + g] = q_inv;
+            __syncwarp();
+        } else {
+            if (warp < NS) {                                           // a slice per warp, through shared memory
+                load_q(warp);
 #pragma unroll
-            for (int x = 0; x < KS; ++x) qf[x] = sm_q[x * 32 + lane];
+                for (int x = 0; x < KS; ++x) sm_q[(warp * KS + x) * 32 + lane] = qf[x];
+                if (t == 0) sm_qinv[warp * 8 + g] = q_inv;
+            }
+            __syncthreads();
         }
         // this thread's query rows are columns 2t, 2t + 1 of each slice
         float qinv[NS * 2], ref[NS * 2], l[NS * 2], acc[NS][KS][4];
@@ -245,7 +269,7 @@ __global__ void __launch_bounds__(PS_THREADS) paged_scan_kernel(const PagedAttnP
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 const int r = r0 + s * 8 + 2 * t + e;
-                qinv[s * 2 + e] = FP8 ? sm_qinv[s * 8 + 2 * t + e] * p.scale_log2 : p.scale_log2;
+                qinv[s * 2 + e] = FP8 ? sm_qinv[(NS == 1 ? warp : s) * 8 + 2 * t + e] * p.scale_log2 : p.scale_log2;
                 last[s * 2 + e] = (int)min((long long)own, len + 1 + (r < rows ? r / p.g : p.m));
                 ref[s * 2 + e] = -INFINITY;
                 l[s * 2 + e] = 0.f;
@@ -258,17 +282,10 @@ __global__ void __launch_bounds__(PS_THREADS) paged_scan_kernel(const PagedAttnP
                 for (int e = 0; e < 4; ++e) acc[s][a][e] = 0.f;
 
         for (int k = 0; k < steps; ++k) {
-            {                                                          // request the step PS_STAGES - 1 ahead
-                int now[SUB];
-#pragma unroll
-                for (int sb = 0; sb < SUB; ++sb) now[sb] = pages[sb];
-                fetch_pages(k + PS_STAGES);
-                if (k + PS_STAGES - 1 < steps) load_step(s0 + warp + (k + PS_STAGES - 1) * PS_WARPS, (k + PS_STAGES - 1) % PS_STAGES, now);
-                else cp_async_commit();
-            }
+            request(k + PS_STAGES - 1);
             cp_async_wait<PS_STAGES - 1>();
             __syncwarp();
-            const uint32_t base = ring + (k % PS_STAGES) * (C::STAGE + C::SC);
+            const uint32_t base = ring + ((k + RED) % PS_STAGES) * (C::STAGE + C::SC);
             const int step = s0 + warp + k * PS_WARPS;
 
             // S^T: two chains of MMAs per tile
@@ -424,8 +441,10 @@ __global__ void __launch_bounds__(PS_THREADS) paged_scan_kernel(const PagedAttnP
             }
             __syncwarp();                                              // the stage may be refilled
         }
-        cp_async_wait<0>();
-        __syncwarp();
+        // every step of this sequence has been consumed: on to the next one that has some in this CTA's piece
+        do ++seq; while (seq < p.b.n_seqs && sm_cnt[seq + 1] <= sm_cnt[seq]);
+        const bool more = seq < p.b.n_seqs && sm_cnt[seq] < hi;
+        if (more) begin();
 
         // ---- join the four warps through their rings and write the piece's partial
 #pragma unroll
@@ -454,7 +473,7 @@ __global__ void __launch_bounds__(PS_THREADS) paged_scan_kernel(const PagedAttnP
                         red[(s * QUADS + (e * VC + c) * PIECES + f) * 32 + lane] = make_float4(acc[s][a][e], acc[s][a][e + 2], acc[s][a + 1][e], acc[s][a + 1][e + 2]);
                     }
         __syncthreads();
-        const long long slot = (long long)hg * (p.ctas + p.b.n_seqs) + blockIdx.x + seq;
+        const long long slot = (long long)hg * (p.ctas + p.b.n_seqs) + blockIdx.x + now;
         for (int x = warp; x < NS * QUADS; x += PS_WARPS) {
             const int s = x / QUADS, e = (x / (VC * PIECES)) & 1, c = (x / PIECES) % VC, f = x % PIECES;
             const int col = s * 8 + 2 * t + e;
@@ -476,57 +495,90 @@ __global__ void __launch_bounds__(PS_THREADS) paged_scan_kernel(const PagedAttnP
                 if (c == 0 && f == 0 && g == 0) *reinterpret_cast<float2 *>(p.part_ml + (slot * 8 * NS + col) * 2) = make_float2(mx, lt);
             }
         }
+        if (!more) break;
         __syncthreads();
     }
+    cp_async_wait<0>();
     pdl_wait();
 }
 
-// Joins the partials of a query row, one warp per row: plan[1] - plan[0] + 1 pieces of the scan, then those of the prefix.  The weights
-// exp2(m - max) are found 32 pieces at a time, one per lane.  Latency-bound: a few KB per row, all from L2.
-template <int D>
+// Joins the partials of a query row: plan[1] - plan[0] + 1 pieces of the scan, then those of the prefix.  WPR warps share a
+// row; each of them finds the weights exp2(m - max) of all pieces, 32 at a time, one per lane, and adds up every
+// WPR-th piece with four of them requested at once.  A few KB per row, from L2: bound by the latency of plan -> (m, l) -> acc.
+template <int D, int WPR>
 __global__ void __launch_bounds__(256) paged_merge_kernel(const PagedAttnParams p, const int ns) {
-    constexpr int EPT = D / 32;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const long long row = (long long)blockIdx.x * 8 + warp;                // (sequence, token, head)
+    constexpr int EPT = D / 32, RPC = 8 / WPR;
+    __shared__ float sm_o[WPR > 1 ? 8 * D : 1];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = warp % WPR;
+    const long long row = (long long)blockIdx.x * RPC + warp / WPR;        // (sequence, token, head)
+    const bool row_ok = row < (long long)p.b.n_seqs * p.m * p.hq;
     pdl_wait();
     pdl_launch_dependents();
-    if (row >= (long long)p.b.n_seqs * p.m * p.hq) return;
-    const int h = (int)(row % p.hq), i = (int)(row / p.hq % p.m), seq = (int)(row / p.hq / p.m);
+    const int h = (int)(row % p.hq), i = (int)(row / p.hq % p.m), seq = row_ok ? (int)(row / p.hq / p.m) : 0;
     const int j = h / p.g, r = i * p.g + h % p.g, grp = r / (8 * ns), col = r % (8 * ns);
-    const int c0 = p.plan[2 * seq], c1 = p.plan[2 * seq + 1];
-    const long long slot0 = ((long long)(grp * p.c.hkv + j) * (p.ctas + p.b.n_seqs) + seq) * 8 * ns + col;
+    const int c0 = p.plan[2 * seq], n_scan = p.plan[2 * seq + 1] - c0 + 1;
+    const int n = !row_ok || load_len(p.b, seq) < 0 ? 0 : n_scan + p.splits;
+    const long long slot0 = ((long long)(grp * p.c.hkv + j) * (p.ctas + p.b.n_seqs) + seq + c0) * 8 * ns + col;
     const long long px0 = ((long long)j * p.b.n_seqs + seq) * p.g * p.m + r, px_step = (long long)p.c.hkv * p.b.n_seqs * p.g * p.m;
     float mx = -INFINITY, l = 0.f, o[EPT];
 #pragma unroll
     for (int e = 0; e < EPT; ++e) o[e] = 0.f;
-    // pieces at part row + x * step, x in [x0, x1]
-    auto join = [&](const float *part_ml, const float *part_acc, long long at, long long step, int x0, int x1) {
-        for (int base = x0; base <= x1; base += 32) {
-            const int n = min(32, x1 - base + 1);
-            float2 ml = make_float2(-INFINITY, 0.f);
-            if (lane < n) ml = *reinterpret_cast<const float2 *>(part_ml + (at + (base + lane) * step) * 2);
-            const float m_new = fmaxf(mx, warp_max(ml.x));
-            const float w = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - m_new);
-            const float alpha = mx == -INFINITY ? 0.f : fast_exp2(mx - m_new);
-            l = l * alpha + warp_sum(ml.y * w);
+    for (int base = 0; base < n; base += 32) {
+        const int x = base + lane;
+        float2 ml = make_float2(-INFINITY, 0.f);
+        const float *acc = nullptr;
+        if (x < n_scan) {
+            const long long at = slot0 + (long long)x * 8 * ns;
+            ml = *reinterpret_cast<const float2 *>(p.part_ml + at * 2);
+            acc = p.part_acc + at * D;
+        } else if (x < n) {
+            const long long at = px0 + (x - n_scan) * px_step;
+            ml = *reinterpret_cast<const float2 *>(p.px_ml + at * 2);
+            acc = p.px_acc + at * D;
+        }
+        const float m_new = fmaxf(mx, warp_max(ml.x));
+        const float w = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - m_new);
+        const float alpha = mx == -INFINITY ? 0.f : fast_exp2(mx - m_new);
+        l = l * alpha + warp_sum(ml.y * w);
 #pragma unroll
-            for (int e = 0; e < EPT; ++e) o[e] *= alpha;
-            mx = m_new;
-            for (int x = 0; x < n; ++x) {
-                const float wx = __shfl_sync(0xffffffffu, w, x);
-                if (__shfl_sync(0xffffffffu, ml.y, x) == 0.f) continue;        // a piece without keys (its acc is not written)
-                const float4 *src = reinterpret_cast<const float4 *>(part_acc + (at + (base + x) * step) * D + lane * EPT);
+        for (int e = 0; e < EPT; ++e) o[e] *= alpha;
+        mx = m_new;
+        if (ml.y == 0.f) acc = nullptr;                                    // a piece without keys: its acc is not written
+        const int here = min(32, n - base);
+        for (int x0 = sub; x0 < here; x0 += 4 * WPR) {
+            float4 v[4][EPT / 4];
+            float wx[4];
+#pragma unroll
+            for (int y = 0; y < 4; ++y) {
+                const int from = x0 + y * WPR;
+                const unsigned long long a = __shfl_sync(0xffffffffu, (unsigned long long)acc, from & 31);
+                wx[y] = __shfl_sync(0xffffffffu, w, from & 31);
+                const bool ok = from < here && a != 0;
+                const float4 *src = reinterpret_cast<const float4 *>(a) + lane * (EPT / 4);
+#pragma unroll
+                for (int e = 0; e < EPT / 4; ++e) v[y][e] = ok ? src[e] : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+#pragma unroll
+            for (int y = 0; y < 4; ++y)
 #pragma unroll
                 for (int e = 0; e < EPT / 4; ++e) {
-                    const float4 v = src[e];
-                    o[e * 4] = fmaf(v.x, wx, o[e * 4]); o[e * 4 + 1] = fmaf(v.y, wx, o[e * 4 + 1]);
-                    o[e * 4 + 2] = fmaf(v.z, wx, o[e * 4 + 2]); o[e * 4 + 3] = fmaf(v.w, wx, o[e * 4 + 3]);
+                    const float wy = x0 + y * WPR < here ? wx[y] : 0.f;
+                    o[e * 4] = fmaf(v[y][e].x, wy, o[e * 4]); o[e * 4 + 1] = fmaf(v[y][e].y, wy, o[e * 4 + 1]);
+                    o[e * 4 + 2] = fmaf(v[y][e].z, wy, o[e * 4 + 2]); o[e * 4 + 3] = fmaf(v[y][e].w, wy, o[e * 4 + 3]);
                 }
-            }
         }
-    };
-    join(p.part_ml, p.part_acc, slot0, 8 * ns, c0, c1);
-    if (p.splits > 0 && load_len(p.b, seq) >= 0) join(p.px_ml, p.px_acc, px0, px_step, 0, p.splits - 1);
+    }
+    if constexpr (WPR > 1) {                                               // the row's warps, in order
+#pragma unroll
+        for (int e = 0; e < EPT; ++e) sm_o[warp * D + e * 32 + lane] = o[e];
+        __syncthreads();
+        if (sub != 0) return;
+#pragma unroll
+        for (int y = 1; y < WPR; ++y)
+#pragma unroll
+            for (int e = 0; e < EPT; ++e) o[e] += sm_o[(warp + y) * D + e * 32 + lane];
+    }
+    if (!row_ok) return;
     const float inv = l == 0.f ? 0.f : __fdiv_rn(1.f, l);                 // a row that sees no key is zero
     __nv_bfloat16 ob[EPT];
 #pragma unroll
@@ -663,8 +715,11 @@ extern "C" int trb_attn_paged(const trb_paged_t *pool, const trb_batch_t *batch,
     else rc = pool->d == 256 ? (fp8 ? launch_scan<ScanCfg<256, true, 2>>(p, st) : launch_scan<ScanCfg<256, false, 2>>(p, st))
                              : (fp8 ? launch_scan<ScanCfg<128, true, 2>>(p, st) : launch_scan<ScanCfg<128, false, 2>>(p, st));
     if (rc) return rc;
+    // few rows: their pieces are many, and eight warps share a row; many rows fill the SMs with a warp each
     const long long out_rows = (long long)batch->n_seqs * a->m * a->hq;
-    TRB_CUDA_CHECK(launch_kernel(pool->d == 256 ? paged_merge_kernel<256> : paged_merge_kernel<128>, dim3((unsigned)((out_rows + 7) / 8)), dim3(256), 0, st,
-                                 true, p, plan.ns));
+    const int wpr = out_rows <= 4LL * sm_count() ? 8 : 1;
+    const dim3 grid((unsigned)((out_rows * wpr + 7) / 8));
+    TRB_CUDA_CHECK(launch_kernel(pool->d == 256 ? (wpr == 8 ? paged_merge_kernel<256, 8> : paged_merge_kernel<256, 1>)
+                                                : (wpr == 8 ? paged_merge_kernel<128, 8> : paged_merge_kernel<128, 1>), grid, dim3(256), 0, st, true, p, plan.ns));
     return TRB_OK;
 }

@@ -6,9 +6,9 @@
 // With one block of rows the kernel is bound by HBM even though the block may be mostly padding (a 128-key e4m3 tile is 64 KB,
 // 1.5 us of an SM's share of HBM, and its MMAs take 1.1 us); with more it is bound by the tensor side.
 //
-// The tile loop is that of the prefill kernel (prefill.cu): S = Q K^T into two alternating tensor-memory buffers, softmax
-// by two warpgroups (thread = one query row and half of a tile's keys), P written over the scores it came from and taken from
-// there as the A operand of O += P V.  e4m3 codes feed kind::f8f6f4 MMAs unconverted, with q and P as hi + lo terms; bf16 pools
+// The tile loop is that of the prefill kernel (prefill.cu): S = Q K^T into two alternating tensor-memory buffers, softmax,
+// P written over the scores it came from and taken from there as the A operand of O += P V.  The softmax pass of a tile is
+// bound by dependency latency, so four warpgroups share it (thread = one query row and a quarter of the keys).  e4m3 codes feed kind::f8f6f4 MMAs unconverted, with q and P as hi + lo terms; bf16 pools
 // feed kind::f16.  Different here: tiles are put together from pages (one TMA box per page and 128-byte column), there is no
 // causal edge, and the rows of the last tile behind the prefix are cleared in shared memory before P V, because pages may hold
 // anything there.
@@ -32,7 +32,7 @@ struct PrefixParams {
     float *part_acc;                   // [splits][hkv][rows][D]
 };
 
-constexpr int PX_BM = 128, PX_SOFTMAX = 256, PX_THREADS = PX_SOFTMAX + 64;
+constexpr int PX_BM = 128, PX_WG = 4, PX_SOFTMAX = PX_WG * 128, PX_WARPS = PX_SOFTMAX / 32, PX_THREADS = PX_SOFTMAX + 64;
 
 template <int D_, bool FP8_> struct PrefixCfg {
     static constexpr int D = D_;
@@ -45,17 +45,18 @@ template <int D_, bool FP8_> struct PrefixCfg {
     static constexpr int OFF_KV = FP8 ? 2 * Q_BYTES : 0;
     static constexpr int OFF_SC = OFF_KV + STAGES * 2 * TILE;          // [SLOTS][2][BN] floats: scales as they lie in the pool
     static constexpr int OFF_FAC = OFF_SC + (FP8 ? SLOTS * 2 * BN * 4 : 0);   // [SLOTS][3][BN] floats: factors of a tile's keys
-    static constexpr int OFF_MX = OFF_FAC + (FP8 ? SLOTS * 3 * BN * 4 : 0);   // [2][2][128] floats: row maxima of the two halves
-    static constexpr int OFF_BAR = OFF_MX + 2 * 2 * PX_BM * 4;
+    static constexpr int OFF_MX = OFF_FAC + (FP8 ? SLOTS * 3 * BN * 4 : 0);   // [2][PX_WG][128] floats: row maxima of the four quarters
+    static constexpr int OFF_BAR = OFF_MX + 2 * PX_WG * PX_BM * 4;
     static constexpr int SMEM = OFF_BAR + 256 + 1024;
     static constexpr int TM_S = 0, TM_O = 256, TM_Q = FP8 ? 0 : (D == 256 ? 128 : 384);
     static_assert(SMEM <= 227 * 1024, "shared memory budget");
+    static_assert(STAGES * 2 * TILE >= PX_BM * D * 4, "the output block is turned in the ring");
 };
 
 template <typename C>
 __global__ void __launch_bounds__(PX_THREADS, 1)
 paged_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const PrefixParams p) {
-    constexpr int D = C::D, BN = C::BN, KPT = BN / 2, SEGS = C::SEGS, TILE = C::TILE, STAGES = C::STAGES, SLOTS = C::SLOTS;
+    constexpr int D = C::D, BN = C::BN, KPT = BN / PX_WG, SEGS = C::SEGS, TILE = C::TILE, STAGES = C::STAGES, SLOTS = C::SLOTS;
     constexpr bool FP8 = C::FP8;
     extern __shared__ uint8_t px_smem_raw[];
     uint8_t *smem = px_smem_raw + ((1024u - (smem_u32(px_smem_raw) & 1023u)) & 1023u);
@@ -82,7 +83,7 @@ paged_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
         }
         for (int b = 0; b < 2; ++b) mbar_init(&s_full[b], 1u);
         for (int b = 0; b < SLOTS; ++b) mbar_init(&fac_full[b], 1u);
-        mbar_init(p_full, 8u); mbar_init(o_done, 1u); mbar_init(o_last, 1u); mbar_init(q_ready, 8u);
+        mbar_init(p_full, PX_WARPS); mbar_init(o_done, 1u); mbar_init(o_last, 1u); mbar_init(q_ready, PX_WARPS);
         mbar_fence_init();
         tma_prefetch_desc(&tm_k); tma_prefetch_desc(&tm_v);
     }
@@ -99,7 +100,7 @@ paged_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
     const int t0 = (int)((long long)split * all_tiles / p.splits), n_tiles = (int)((long long)(split + 1) * all_tiles / p.splits) - t0;
     const int left_last = n_prefix - (t0 + n_tiles - 1) * BN;           // keys of this piece's last tile (>= BN: it is whole)
 
-    if (warp == 8) {
+    if (warp == PX_WARPS) {
         // ================================ TMA producer ================================
         // lane x holds the page of the x-th 16 keys of the tile; it is requested a tile ahead
         const int page_mask = (1 << p.c.page_shift) - 1;
@@ -125,7 +126,7 @@ paged_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
             if (lane == 0) mbar_arrive(&fac_full[t % SLOTS]);
             return true;
         };
-        int next = page_at(0);
+        int next = page_at(0), k_sent = 0, v_sent = 0;
         for (int i = 0; i < n_tiles; ++i) {
             const int s = i % STAGES, row0 = (t0 + i) * BN;
             int page = next;
@@ -149,6 +150,7 @@ paged_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
             };
             if (i >= STAGES && !mbar_wait(&k_free[s], par)) break;                 // the product with the stage's last K tile has run
             load(kt, &tm_k, &k_full[s]);
+            ++k_sent;
             if constexpr (FP8) {
                 float *sc = sm_sc + (i % SLOTS) * 2 * BN;
 #pragma unroll
@@ -164,9 +166,13 @@ paged_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
             }
             if (i >= STAGES && !mbar_wait(&v_free[s], par)) break;
             load(vt, &tm_v, &v_full[s]);
+            ++v_sent;
         }
         if constexpr (FP8) { if (n_tiles > 0) build_factors(n_tiles - 1); }
-    } else if (warp == 9) {
+        // no copy is on its way when the CTA leaves, also after a wait that ran out
+        for (int t = max(0, k_sent - STAGES); t < k_sent; ++t) mbar_wait(&k_full[t % STAGES], (t / STAGES) & 1);
+        for (int t = max(0, v_sent - STAGES); t < v_sent; ++t) mbar_wait(&v_full[t % STAGES], (t / STAGES) & 1);
+    } else if (warp == PX_WARPS + 1) {
         // ================================ MMA issuer ==================================
         // QK(0), QK(1), PV(0), QK(2), PV(1), ..: the pipe runs in order of issue, so QK(i + 2) overwrites the buffer that holds
         // P(i) only after PV(i) has read it
@@ -240,69 +246,87 @@ paged_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
             __syncwarp();
         }
     } else {
-        // ============ softmax / correction / epilogue: warps 0-7, thread = (row, half of the keys) ============
-        const int row = (warp & 3) * 32 + lane, half = warp >> 2;                  // query row = TMEM lane
+        // ============ softmax / correction / epilogue: thread = (row, quarter of the keys and of the output columns) ============
+        const int row = (warp & 3) * 32 + lane, part = warp >> 2;                  // query row = TMEM lane
         const bool row_ok = row < rows_here, warp_ok = (warp & 3) * 32 < rows_here;
         const int rr = q0 + (row_ok ? row : 0), seq = rr / rows_seq, r = rr % rows_seq;
-        const __nv_bfloat16 *qp = p.q + (((long long)seq * p.m + r / p.g) * p.hq + j * p.g + r % p.g) * D;
+        const long long q_off = (((long long)seq * p.m + r / p.g) * p.hq + j * p.g + r % p.g) * D;
         const uint32_t lane_addr = tmem + ((uint32_t)((warp & 3) * 32) << 16);
         float qinv = 1.f;
         if (n_tiles > 0) {
             if constexpr (!FP8) {
-                // two dims per column, this thread's half of the row; rows past the last are zero
+                // two dims per column, this thread's quarter of the row; rows past the last are zero
+                const uint4 *qp = reinterpret_cast<const uint4 *>(p.q + q_off + part * (D / PX_WG));
+                uint32_t w[D / PX_WG / 2];
 #pragma unroll
-                for (int blk32 = 0; blk32 < D / 128; ++blk32) {
-                    uint32_t w[32];
-#pragma unroll
-                    for (int c = 0; c < 8; ++c) {
-                        const uint4 raw = row_ok ? *reinterpret_cast<const uint4 *>(qp + half * (D / 2) + blk32 * 64 + c * 8) : make_uint4(0u, 0u, 0u, 0u);
-                        w[c * 4 + 0] = raw.x; w[c * 4 + 1] = raw.y; w[c * 4 + 2] = raw.z; w[c * 4 + 3] = raw.w;
-                    }
-                    tmem_st32_raw(lane_addr + C::TM_Q + half * (D / 4) + blk32 * 32, w);
+                for (int c = 0; c < D / PX_WG / 8; ++c) {
+                    const uint4 raw = row_ok ? qp[c] : make_uint4(0u, 0u, 0u, 0u);
+                    w[c * 4 + 0] = raw.x; w[c * 4 + 1] = raw.y; w[c * 4 + 2] = raw.z; w[c * 4 + 3] = raw.w;
                 }
+                if constexpr (D == 256) tmem_st32_raw(lane_addr + C::TM_Q + part * 32, w);
+                else tmem_st16_raw(lane_addr + C::TM_Q + part * 16, w);
                 tmem_st_wait();
             } else {
-                // hi + lo e4m3 copies with a power-of-two factor for the row
-                float amax = 0.f;
-                for (int c = 0; c < D / 8; ++c) {
-                    const uint4 raw = *reinterpret_cast<const uint4 *>(qp + c * 8);
-                    const __nv_bfloat162 *b2 = reinterpret_cast<const __nv_bfloat162 *>(&raw);
+                // hi + lo e4m3 copies with a power-of-two factor for the row.  A warp takes 8 rows, D / 8 lanes with 16 bytes each per row,
+                // all requested at once: read by the thread that owns the row, the block took most of 20 us
+                long long *sm_off = reinterpret_cast<long long *>(sm_mx);          // [128], then the factors behind it: both are read before tile 0 writes here
+                float *sm_qinv = sm_mx + 2 * PX_BM;
+                if (part == 0) sm_off[row] = row_ok ? q_off : -1;
+                named_barrier(1, PX_SOFTMAX);
+                constexpr int LPR = D / 8, RPL = 32 / LPR, LOADS = PX_BM / PX_WARPS / RPL;
+                uint4 raw[LOADS];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) { const float2 f = __bfloat1622float2(b2[e]); amax = fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y))); }
+                for (int x = 0; x < LOADS; ++x) {
+                    const long long off = sm_off[warp * (PX_BM / PX_WARPS) + x * RPL + lane / LPR];
+                    raw[x] = off >= 0 ? *reinterpret_cast<const uint4 *>(p.q + off + lane % LPR * 8) : make_uint4(0u, 0u, 0u, 0u);
                 }
-                int e = (int)((__float_as_uint(amax) >> 23) & 0xffu) - 127;
-                if (amax == 0.f || e < -90 || !row_ok) e = 7;
-                if (e > 90) e = 90;
-                const float sc = row_ok ? __uint_as_float((uint32_t)(127 + 7 - e) << 23) : 0.f;
-                qinv = __uint_as_float((uint32_t)(127 - 7 + e) << 23);
-                for (int cc = 0; cc < D / 32; ++cc) {
-                    const int c = half * (D / 32) + cc;
-                    uint32_t hw[4], lw[4];
 #pragma unroll
-                    for (int w = 0; w < 4; ++w) {
-                        const uint2 raw = *reinterpret_cast<const uint2 *>(qp + c * 16 + w * 4);
-                        const float2 a = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&raw.x));
-                        const float2 b = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&raw.y));
-                        const float y[4] = {a.x * sc, a.y * sc, b.x * sc, b.y * sc};
+                for (int x = 0; x < LOADS; ++x) {
+                    const int wr = warp * (PX_BM / PX_WARPS) + x * RPL + lane / LPR;
+                    const __nv_bfloat162 *b2 = reinterpret_cast<const __nv_bfloat162 *>(&raw[x]);
+                    float f[8], amax = 0.f;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float2 v = __bfloat1622float2(b2[e]);
+                        f[2 * e] = v.x; f[2 * e + 1] = v.y;
+                        amax = fmaxf(amax, fmaxf(fabsf(v.x), fabsf(v.y)));
+                    }
+#pragma unroll
+                    for (int o = LPR / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+                    int e = (int)((__float_as_uint(amax) >> 23) & 0xffu) - 127;
+                    if (amax == 0.f || e < -90) e = 7;
+                    if (e > 90) e = 90;
+                    const float sc = __uint_as_float((uint32_t)(127 + 7 - e) << 23);
+                    if (lane % LPR == 0) sm_qinv[wr] = __uint_as_float((uint32_t)(127 - 7 + e) << 23);
+                    uint32_t hw[2], lw[2];
+#pragma unroll
+                    for (int w = 0; w < 2; ++w) {
+                        const float y[4] = {f[4 * w] * sc, f[4 * w + 1] * sc, f[4 * w + 2] * sc, f[4 * w + 3] * sc};
                         pf_split4(y, hw[w], lw[w]);
                     }
-                    const uint32_t off = (c >> 3) * (PX_BM * 128) + sw128(row, (c & 7) * 16);
-                    *reinterpret_cast<uint4 *>(smem + off) = make_uint4(hw[0], hw[1], hw[2], hw[3]);
-                    *reinterpret_cast<uint4 *>(smem + C::Q_BYTES + off) = make_uint4(lw[0], lw[1], lw[2], lw[3]);
+                    const int byte = lane % LPR * 8;
+                    const uint32_t off = (byte >> 7) * (PX_BM * 128) + sw128(wr, byte & 127);
+                    *reinterpret_cast<uint2 *>(smem + off) = make_uint2(hw[0], hw[1]);
+                    *reinterpret_cast<uint2 *>(smem + C::Q_BYTES + off) = make_uint2(lw[0], lw[1]);
                 }
                 fence_async_smem();
             }
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(q_ready);
+            if constexpr (FP8) {
+                named_barrier(1, PX_SOFTMAX);
+                qinv = sm_mx[2 * PX_BM + row];
+                named_barrier(1, PX_SOFTMAX);                                      // (read by all before a tile's maxima are written over it)
+            }
         }
 
-        float m_run = -INFINITY, l_run = 0.f;                                      // l_run: this thread's half of the keys
+        float m_run = -INFINITY, l_run = 0.f;                                      // l_run: this thread's quarter of the keys
         bool ok = true;
         for (int i = 0; i < n_tiles; ++i) {
             const int b = i & 1;
-            const float *fac = sm_fac + (i % SLOTS) * 3 * BN + half * KPT;
-            float *mxbuf = sm_mx + b * 2 * PX_BM;
+            const float *fac = sm_fac + (i % SLOTS) * 3 * BN + part * KPT;
+            float *mxbuf = sm_mx + b * PX_WG * PX_BM;
             ok = ok && mbar_wait(&s_full[b], (i >> 1) & 1);
             if constexpr (FP8) ok = ok && mbar_wait(&fac_full[i % SLOTS], (i / SLOTS) & 1);
             ok = __all_sync(0xffffffffu, ok);
@@ -310,9 +334,8 @@ paged_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
             // a warp without query rows, or one whose wait ran out, only takes part in the barriers
             if (warp_ok && ok) {
                 float sv[KPT];
-#pragma unroll
-                for (int c = 0; c < KPT / 32; ++c)
-                    tmem_ld32(lane_addr + C::TM_S + b * BN + half * KPT + c * 32, *reinterpret_cast<float (*)[32]>(&sv[c * 32]));
+                if constexpr (KPT == 32) tmem_ld32(lane_addr + C::TM_S + b * BN + part * KPT, sv);
+                else tmem_ld16(lane_addr + C::TM_S + b * BN + part * KPT, sv);
                 if constexpr (!FP8) {
                     const float2 sl2 = make_float2(p.scale_log2, p.scale_log2);
 #pragma unroll
@@ -334,16 +357,14 @@ paged_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
                 if (i == n_tiles - 1 && left_last < BN) {
 #pragma unroll
                     for (int c = 0; c < KPT; ++c)
-                        if (half * KPT + c >= left_last) sv[c] = -INFINITY;
+                        if (part * KPT + c >= left_last) sv[c] = -INFINITY;
                 }
                 float mt4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
                 for (int c = 0; c < KPT / 2; ++c) mt4[c & 3] = pf_max3(mt4[c & 3], sv[2 * c], sv[2 * c + 1]);
-                float mt = fmaxf(fmaxf(mt4[0], mt4[1]), fmaxf(mt4[2], mt4[3]));
-                mxbuf[half * PX_BM + row] = mt;
+                mxbuf[part * PX_BM + row] = fmaxf(fmaxf(mt4[0], mt4[1]), fmaxf(mt4[2], mt4[3]));
                 named_barrier(1, PX_SOFTMAX);
-                mt = fmaxf(mt, mxbuf[(half ^ 1) * PX_BM + row]);
-                const float m_new = fmaxf(m_run, mt);
+                const float m_new = fmaxf(pf_max3(m_run, mxbuf[row], mxbuf[PX_BM + row]), fmaxf(mxbuf[2 * PX_BM + row], mxbuf[3 * PX_BM + row]));
                 const float m_safe = m_new == -INFINITY ? 0.f : m_new;
                 const float m_off = FP8 ? m_safe - 8.f : m_safe;                   // e4m3 weights are staged x 256
                 const float alpha = m_new == -INFINITY ? 1.f : fast_exp2(m_run - m_safe);
@@ -354,54 +375,49 @@ paged_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
                     if (ok) {
                         tc_fence_after();
 #pragma unroll 1
-                        for (int c = 0; c < D / 64; ++c) {
+                        for (int c = 0; c < D / PX_WG / 32; ++c) {
                             float ov[32];
-                            tmem_ld32(lane_addr + C::TM_O + half * (D / 2) + c * 32, ov);
+                            tmem_ld32(lane_addr + C::TM_O + part * (D / PX_WG) + c * 32, ov);
 #pragma unroll
                             for (int e = 0; e < 32; ++e) ov[e] *= alpha;
-                            tmem_st32(lane_addr + C::TM_O + half * (D / 2) + c * 32, ov);
+                            tmem_st32(lane_addr + C::TM_O + part * (D / PX_WG) + c * 32, ov);
                         }
                     }
                 }
                 const uint32_t p_tm = lane_addr + C::TM_S + b * BN;                // (all of S was read before the barrier above)
                 float lsum = 0.f;
                 if constexpr (!FP8) {
+                    uint32_t w[KPT / 2];
 #pragma unroll
-                    for (int x = 0; x < KPT / 32; ++x) {
-                        uint32_t w[16];
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) {
-                            w[e] = pack_bf16x2(fast_exp2(sv[x * 32 + e * 2] - m_off), fast_exp2(sv[x * 32 + e * 2 + 1] - m_off));
-                            const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&w[e]));   // the sum takes the weights as they multiply V
-                            lsum += f.x + f.y;
-                        }
-                        tmem_st16_raw(p_tm + half * (KPT / 2) + x * 16, w);
+                    for (int e = 0; e < KPT / 2; ++e) {
+                        w[e] = pack_bf16x2(fast_exp2(sv[e * 2] - m_off), fast_exp2(sv[e * 2 + 1] - m_off));
+                        const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&w[e]));   // the sum takes the weights as they multiply V
+                        lsum += f.x + f.y;
                     }
+                    if constexpr (KPT == 32) tmem_st16_raw(p_tm + part * 16, w);
+                    else tmem_st8_raw(p_tm + part * 8, w);
                 } else {
                     const float2 nm2 = make_float2(-m_off, -m_off);
                     float2 lsa = make_float2(0.f, 0.f), lsb = make_float2(0.f, 0.f);
+                    uint32_t hw8[8], lw8[8];
 #pragma unroll
-                    for (int g32 = 0; g32 < KPT / 32; ++g32) {
-                        uint32_t hw8[8], lw8[8];
-#pragma unroll
-                        for (int w = 0; w < 8; ++w) {
-                            const int k0 = g32 * 32 + w * 4;
-                            const float4 fr = *reinterpret_cast<const float4 *>(fac + 2 * BN + k0);
-                            const float2 d01 = __fadd2_rn(make_float2(sv[k0 + 0], sv[k0 + 1]), nm2);
-                            const float2 d23 = __fadd2_rn(make_float2(sv[k0 + 2], sv[k0 + 3]), nm2);
-                            const float2 p01 = make_float2(fast_exp2(d01.x), fast_exp2(d01.y));
-                            const float2 p23 = make_float2(fast_exp2(d23.x), fast_exp2(d23.y));
-                            lsa = __ffma2_rn(p01, make_float2(fr.x, fr.y), lsa);
-                            lsb = __ffma2_rn(p23, make_float2(fr.z, fr.w), lsb);
-                            uint32_t h01, l01, h23, l23;
-                            pf_split2_h(p01.x, p01.y, h01, l01);
-                            pf_split2_h(p23.x, p23.y, h23, l23);
-                            hw8[w] = h01 | (h23 << 16);
-                            lw8[w] = l01 | (l23 << 16);
-                        }
-                        tmem_st8_raw(p_tm + half * (KPT / 4) + g32 * 8, hw8);
-                        tmem_st8_raw(p_tm + BN / 4 + half * (KPT / 4) + g32 * 8, lw8);
+                    for (int w = 0; w < 8; ++w) {
+                        const int k0 = w * 4;
+                        const float4 fr = *reinterpret_cast<const float4 *>(fac + 2 * BN + k0);
+                        const float2 d01 = __fadd2_rn(make_float2(sv[k0 + 0], sv[k0 + 1]), nm2);
+                        const float2 d23 = __fadd2_rn(make_float2(sv[k0 + 2], sv[k0 + 3]), nm2);
+                        const float2 p01 = make_float2(fast_exp2(d01.x), fast_exp2(d01.y));
+                        const float2 p23 = make_float2(fast_exp2(d23.x), fast_exp2(d23.y));
+                        lsa = __ffma2_rn(p01, make_float2(fr.x, fr.y), lsa);
+                        lsb = __ffma2_rn(p23, make_float2(fr.z, fr.w), lsb);
+                        uint32_t h01, l01, h23, l23;
+                        pf_split2_h(p01.x, p01.y, h01, l01);
+                        pf_split2_h(p23.x, p23.y, h23, l23);
+                        hw8[w] = h01 | (h23 << 16);
+                        lw8[w] = l01 | (l23 << 16);
                     }
+                    tmem_st8_raw(p_tm + part * 8, hw8);
+                    tmem_st8_raw(p_tm + BN / 4 + part * 8, lw8);
                     lsum = (lsa.x + lsa.y) + (lsb.x + lsb.y);
                 }
                 l_run = fmaf(l_run, alpha, lsum);
@@ -417,23 +433,35 @@ paged_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
         // ---- the piece's partial.  The last PV has a barrier of its own: a warp that skipped corrections does not know how many phases
         // of o_done have passed, so no parity of it would name the last one
         if (ok && n_tiles > 0) ok = mbar_wait(o_last, 0);
+        ok = __all_sync(0xffffffffu, ok);
         tc_fence_after();
-        sm_mx[half * PX_BM + row] = l_run;
-        named_barrier(1, PX_SOFTMAX);
-        const float l_tot = l_run + sm_mx[(half ^ 1) * PX_BM + row];
-        const long long at = ((long long)split * p.c.hkv + j) * rows_all + q0 + row;
-        if (row_ok && half == 0)                                                   // weights carry 2^8 with e4m3
-            *reinterpret_cast<float2 *>(p.part_ml + at * 2) = make_float2(FP8 ? m_run - 8.f : m_run, l_tot);
+        // O goes through the ring (every tile has been consumed), so that it leaves in whole rows: 16-byte pieces, swizzled by row
+        float4 *sm_o = reinterpret_cast<float4 *>(smem + C::OFF_KV);
+        float *sm_l = sm_mx + (n_tiles & 1) * PX_WG * PX_BM;                       // (the other buffer may still be read)
+        sm_l[part * PX_BM + row] = l_run;
         if (n_tiles > 0 && warp_ok) {
 #pragma unroll 1
-            for (int c = 0; c < D / 64; ++c) {
+            for (int c = 0; c < D / PX_WG / 32; ++c) {
                 float ov[32];
-                tmem_ld32(lane_addr + C::TM_O + half * (D / 2) + c * 32, ov);
-                if (row_ok) {
-                    float4 *dst = reinterpret_cast<float4 *>(p.part_acc + at * D + half * (D / 2) + c * 32);
+                tmem_ld32(lane_addr + C::TM_O + part * (D / PX_WG) + c * 32, ov);
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) dst[e] = make_float4(ov[e * 4], ov[e * 4 + 1], ov[e * 4 + 2], ov[e * 4 + 3]);
+                for (int e = 0; e < 8; ++e) {
+                    const int piece = part * (D / PX_WG / 4) + c * 8 + e;
+                    sm_o[row * (D / 4) + (piece ^ (row & 7))] = make_float4(ov[e * 4], ov[e * 4 + 1], ov[e * 4 + 2], ov[e * 4 + 3]);
                 }
+            }
+        }
+        named_barrier(1, PX_SOFTMAX);
+        const long long at = ((long long)split * p.c.hkv + j) * rows_all + q0;
+        if (row_ok && part == 0)                                                   // weights carry 2^8 with e4m3
+            *reinterpret_cast<float2 *>(p.part_ml + (at + row) * 2) =
+                make_float2(FP8 ? m_run - 8.f : m_run, (sm_l[row] + sm_l[PX_BM + row]) + (sm_l[2 * PX_BM + row] + sm_l[3 * PX_BM + row]));
+        if (n_tiles > 0) {
+            float4 *dst = reinterpret_cast<float4 *>(p.part_acc + at * D);
+#pragma unroll 4
+            for (int x = warp * 32 + lane; x < rows_here * (D / 4); x += PX_SOFTMAX) {
+                const int orow = x / (D / 4), piece = x % (D / 4);
+                dst[x] = sm_o[orow * (D / 4) + (piece ^ (orow & 7))];
             }
         }
         tc_fence_before();
