@@ -334,41 +334,60 @@ def cursor_advance(pos_t, delta: int):
 
 # ------------------------------------------------------------------------------ batches over a paged cache
 
-def _on_device(*ts) -> int:
+_BF16, _F32, _F64, _I32, _I64, _E4M3 = torch.bfloat16, torch.float32, torch.float64, torch.int32, torch.int64, torch.float8_e4m3fn
+_pack_pool, _pack_batch, _pack_append = L.packer(L.Paged), L.packer(L.Batch), L.packer(L.PagedAppendArgs)
+_pack_attn, _pack_verify = L.packer(L.AttnPagedArgs), L.packer(L.SpecVerifyArgs)
+_attn_workspace: dict = {}           # geometry -> bytes
+
+
+def _on_device(first, *ts) -> int:
     """The index of the current device, which all the tensors given have to be on."""
-    for t in ts:
-        if t is not None and not t.is_cuda:
-            raise RuntimeError("tokenrush_b200 runs on CUDA tensors only (there is no CPU path)")
-    index = torch.cuda.current_device()
+    index = first.get_device()
     for t in ts:
         if t is not None and t.get_device() != index:
-            raise RuntimeError(f"a tensor is on cuda:{t.get_device()}, the current device is cuda:{index}")
+            index = -1
+    if index < 0:
+        raise RuntimeError("tokenrush_b200 runs on CUDA tensors only (there is no CPU path), and on one device in a call")
+    if index != torch.cuda.current_device():
+        raise RuntimeError(f"the tensors are on cuda:{index}, the current device is cuda:{torch.cuda.current_device()}")
     return index
 
 
-def _pool(k_pages, v_pages, k_scale, v_scale) -> L.Paged:
-    """One layer's pool of pages [PAGES, HKV, PAGE, D] (+ scales [PAGES, HKV, PAGE] for fp8)."""
-    shape = k_pages.shape
-    if len(shape) != 4 or v_pages.shape != shape or not k_pages.is_contiguous() or not v_pages.is_contiguous():
+def _pool(k_pages, v_pages, k_scale, v_scale):
+    """One layer's pool of pages [PAGES, HKV, PAGE, D] (+ scales [PAGES, HKV, PAGE] for fp8): (trb_paged_t, its shape)."""
+    shape, kind = k_pages.shape, k_pages.dtype
+    if len(shape) != 4 or v_pages.shape != shape or not (k_pages.is_contiguous() and v_pages.is_contiguous()):
         raise ValueError("pools must be contiguous [PAGES, HKV, PAGE, D] of one shape")
-    fp8 = k_pages.dtype == torch.float8_e4m3fn
-    if v_pages.dtype != k_pages.dtype or not (fp8 or k_pages.dtype == torch.bfloat16):
+    if v_pages.dtype is not kind or not (kind is _E4M3 or kind is _BF16):
         raise TypeError("pools must be float8_e4m3fn or bfloat16")
-    ks = vs = None
-    if fp8:
-        for t in (k_scale, v_scale):
-            if t is None or t.dtype != torch.float32 or t.shape != shape[:3] or not t.is_contiguous():
-                raise ValueError("an fp8 pool needs contiguous float32 k_scale and v_scale [PAGES, HKV, PAGE]")
-        ks, vs = k_scale.data_ptr(), v_scale.data_ptr()
-    return L.Paged(k_pages.data_ptr(), v_pages.data_ptr(), ks, vs, shape[1], shape[3], L.TRB_KV_FP8 if fp8 else L.TRB_KV_BF16, shape[2], shape[0])
+    pages, hkv, page, d = shape
+    if kind is _BF16:
+        return _pack_pool(k_pages.data_ptr(), v_pages.data_ptr(), 0, 0, hkv, d, L.TRB_KV_BF16, page, pages), shape
+    if (k_scale is None or v_scale is None or k_scale.dtype is not _F32 or v_scale.dtype is not _F32 or k_scale.shape != shape[:3]
+            or v_scale.shape != shape[:3] or not (k_scale.is_contiguous() and v_scale.is_contiguous())):
+        raise ValueError("an fp8 pool needs contiguous float32 k_scale and v_scale [PAGES, HKV, PAGE]")
+    return _pack_pool(k_pages.data_ptr(), v_pages.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), hkv, d, L.TRB_KV_FP8, page, pages), shape
 
 
-def _batch(table, lens) -> L.Batch:
-    if table.dtype != torch.int32 or table.dim() != 2 or table.stride(1) != 1:
+def _batch(table, lens):
+    """(trb_batch_t, number of sequences)"""
+    shape, stride, kind = table.shape, table.stride(), lens.dtype
+    if table.dtype is not _I32 or len(shape) != 2 or stride[1] != 1:
         raise ValueError("table must be int32 [B, PAGES] with contiguous rows")
-    if lens.dtype not in (torch.int32, torch.int64) or lens.dim() != 1 or lens.shape[0] != table.shape[0] or not lens.is_contiguous():
+    if not (kind is _I64 or kind is _I32) or lens.shape != shape[:1] or not lens.is_contiguous():
         raise ValueError("lens must be contiguous int32 or int64 [B]")
-    return L.Batch(table.data_ptr(), table.stride(0), lens.data_ptr(), lens.element_size(), table.shape[0], table.shape[1], 0)
+    return _pack_batch(table.data_ptr(), stride[0], lens.data_ptr(), 8 if kind is _I64 else 4, shape[0], shape[1], 0), shape[0]
+
+
+def _length(x, index):
+    """The fields of a trb_cursor_t: a python int, or a device tensor of one int32 / int64."""
+    if not isinstance(x, torch.Tensor):
+        return 0, 8, 0, int(x)
+    if not (x.dtype is _I64 or x.dtype is _I32) or x.numel() != 1:
+        raise TypeError("a length on the device is an int32 or int64 tensor of one element")
+    if x.get_device() != index:
+        raise RuntimeError("the length is not on the device of the other tensors")
+    return x.data_ptr(), 8 if x.dtype is _I64 else 4, 0, 0
 
 
 def paged_append(k, v, k_pages, v_pages, table, lens, k_scale=None, v_scale=None, *, q=None, cu=None, base=0, q_norm_w=None, k_norm_w=None,
@@ -382,40 +401,51 @@ def paged_append(k, v, k_pages, v_pages, table, lens, k_scale=None, v_scale=None
     interleaved, (2x, 2x + 1).  Returns the finished q [T, HQ, D] (None without q).  Two sequences of one call must not
     share the pages they write."""
     index = _on_device(k, v, k_pages, v_pages, k_scale, v_scale, table, lens, q, cu, q_norm_w, k_norm_w, inv_freq)
-    pool, batch = _pool(k_pages, v_pages, k_scale, v_scale), _batch(table, lens)
-    t, d = k.shape[0], pool.d
-    if k.dim() != 3 or k.shape[1] != pool.hkv or k.shape[2] != d or v.shape != k.shape:
+    pool, shape = _pool(k_pages, v_pages, k_scale, v_scale)
+    batch, b = _batch(table, lens)
+    hkv, d, ks, vs = shape[1], shape[3], k.stride(), v.stride()
+    kshape = k.shape
+    t = kshape[0]
+    if kshape != (t, hkv, d) or v.shape != kshape:
         raise ValueError("k and v must be [T, HKV, D] of the pool's heads")
-    for x in (k, v, q):
-        if x is not None and (x.dtype != torch.bfloat16 or x.stride(-1) != 1):
-            raise ValueError("q, k, v must be bfloat16 with a contiguous last dim")
-    for w in (q_norm_w, k_norm_w):
-        if w is not None and (w.dtype != torch.bfloat16 or w.shape != (d,) or not w.is_contiguous()):
-            raise ValueError("norm weights must be bfloat16 [D]")
-    b, rows, rd = batch.n_seqs, 0, 0
-    if cu is None:
-        if t % b:
-            raise ValueError("without cu every sequence has the same number of rows")
-        rows = t // b
-    elif cu.dtype != torch.int32 or cu.shape != (b + 1,) or not cu.is_contiguous():
-        raise ValueError("cu must be int32 [B + 1]")
-    if inv_freq is not None:
-        if inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 or not inv_freq.is_contiguous():
-            raise ValueError("inv_freq must be float64 [rotary_dim / 2]")
-        rd = 2 * inv_freq.shape[0]
-    out = None
+    if k.dtype is not _BF16 or v.dtype is not _BF16 or ks[2] != 1 or vs[2] != 1:
+        raise ValueError("k and v must be bfloat16 with a contiguous last dim")
+    out, qs, qp, op, hq = None, (0, 0), 0, 0, 0
     if q is not None:
-        if q.dim() != 3 or q.shape[0] != t or q.shape[2] != d:
-            raise ValueError("q must be [T, HQ, D]")
-        out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+        qshape, qs = q.shape, q.stride()
+        if len(qshape) != 3 or qshape[0] != t or qshape[2] != d or q.dtype is not _BF16 or qs[2] != 1:
+            raise ValueError("q must be bfloat16 [T, HQ, D] with a contiguous last dim")
+        hq = qshape[1]
+        out = q.new_empty(qshape)
+        qp, op = q.data_ptr(), out.data_ptr()
+    qw = kw = cup = rows = fp = rd = 0
+    if q_norm_w is not None:
+        if q_norm_w.dtype is not _BF16 or q_norm_w.shape != (d,) or not q_norm_w.is_contiguous():
+            raise ValueError("norm weights must be bfloat16 [D]")
+        qw = q_norm_w.data_ptr()
+    if k_norm_w is not None:
+        if k_norm_w.dtype is not _BF16 or k_norm_w.shape != (d,) or not k_norm_w.is_contiguous():
+            raise ValueError("norm weights must be bfloat16 [D]")
+        kw = k_norm_w.data_ptr()
+    if cu is None:
+        rows = t // b if b else 0
+        if rows * b != t:
+            raise ValueError("without cu every sequence has the same number of rows")
+    else:
+        if cu.dtype is not _I32 or cu.shape != (b + 1,) or not cu.is_contiguous():
+            raise ValueError("cu must be int32 [B + 1]")
+        cup = cu.data_ptr()
+    if inv_freq is not None:
+        if inv_freq.dtype is not _F64 or inv_freq.dim() != 1 or not inv_freq.is_contiguous():
+            raise ValueError("inv_freq must be float64 [rotary_dim / 2]")
+        fp, rd = inv_freq.data_ptr(), 2 * inv_freq.shape[0]
     if t == 0:
         return out
-    a = L.PagedAppendArgs(q.data_ptr() if q is not None else None, k.data_ptr(), v.data_ptr(), out.data_ptr() if q is not None else None,
-                          q.stride(0) if q is not None else 0, q.stride(1) if q is not None else 0, k.stride(0), k.stride(1), v.stride(0), v.stride(1),
-                          q_norm_w.data_ptr() if q_norm_w is not None else None, k_norm_w.data_ptr() if k_norm_w is not None else None,
-                          inv_freq.data_ptr() if rd else None, cu.data_ptr() if cu is not None else None, t, rows, q.shape[1] if q is not None else 0,
-                          rd, int(interleaved), eps, amplitude, _cursor(base))
-    L.check(L.lib().trb_paged_append(C.byref(pool), C.byref(batch), C.byref(a), torch._C._cuda_getCurrentRawStream(index)), "trb_paged_append")
+    a = _pack_append(qp, k.data_ptr(), v.data_ptr(), op, qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], qw, kw, fp, cup, t, rows, hq, rd, 1 if interleaved else 0,
+                     eps, amplitude, *_length(base, index))
+    code = L.lib().trb_paged_append(pool, batch, a, torch._C._cuda_getCurrentRawStream(index))
+    if code:
+        raise L.TrbError(code, "trb_paged_append")
     return out
 
 
@@ -426,38 +456,47 @@ def attn_paged(q, k_pages, v_pages, table, lens, k_scale=None, v_scale=None, *, 
     lens[b] < 0 give zeros.  gate (optional): bf16 [B, M, HQ, D] view, out = bf16(o) * bf16(sigmoid(gate)) as in attn_decode_fused.
     Returns [B, M, HQ, D].  Lengths are read on the device, so a captured step serves all of them."""
     index = _on_device(q, k_pages, v_pages, k_scale, v_scale, table, lens, prefix_table, gate, out)
-    pool, batch = _pool(k_pages, v_pages, k_scale, v_scale), _batch(table, lens)
+    pool, pshape = _pool(k_pages, v_pages, k_scale, v_scale)
+    batch, b = _batch(table, lens)
     shape = q.shape
-    if len(shape) != 4 or shape[0] != batch.n_seqs or shape[3] != pool.d or q.dtype != torch.bfloat16 or not q.is_contiguous():
+    if len(shape) != 4 or shape[0] != b or shape[3] != pshape[3] or q.dtype is not _BF16 or not q.is_contiguous():
         raise ValueError("q must be contiguous bf16 [B, M, HQ, D]")
-    m, hq, pages = shape[1], shape[2], 0
+    m, hq, d, pages, pt = shape[1], shape[2], shape[3], 0, 0
     if prefix_table is not None:
-        if prefix_table.dtype != torch.int32 or prefix_table.dim() != 1 or not prefix_table.is_contiguous():
+        if prefix_table.dtype is not _I32 or prefix_table.dim() != 1 or not prefix_table.is_contiguous():
             raise ValueError("prefix_table must be contiguous int32 [P]")
         pages = prefix_table.shape[0]
-        if not isinstance(prefix_len, torch.Tensor) and not 0 <= prefix_len <= pages * pool.page_size:
+        if not isinstance(prefix_len, torch.Tensor) and not 0 <= prefix_len <= pages * pshape[2]:
             raise ValueError("prefix_len exceeds the pages of prefix_table")
+        pt = prefix_table.data_ptr() if pages else 0
     elif isinstance(prefix_len, torch.Tensor) or prefix_len != 0:
         raise ValueError("a prefix needs its prefix_table")
-    rs = hs = 0
+    rs = hs = gp = 0
     if gate is not None:
-        if gate.shape != shape or gate.dtype != torch.bfloat16 or gate.stride(3) != 1 or gate.stride(0) != m * gate.stride(1):
+        if gate.shape != shape or gate.dtype is not _BF16 or gate.stride(3) != 1 or gate.stride(0) != m * gate.stride(1):
             raise ValueError("gate must be a bf16 [B, M, HQ, D] view with equally spaced rows")
-        rs, hs = gate.stride(1), gate.stride(2)
+        rs, hs, gp = gate.stride(1), gate.stride(2), gate.data_ptr()
     if out is None:
-        out = torch.empty(shape, device=q.device, dtype=q.dtype)
-    elif out.shape != shape or out.dtype != torch.bfloat16 or not out.is_contiguous():
+        out = q.new_empty(shape)
+    elif out.shape != shape or out.dtype is not _BF16 or not out.is_contiguous():
         raise ValueError("out must be contiguous bf16 [B, M, HQ, D]")
     lib = L.lib()
-    n = lib.trb_attn_paged_workspace_bytes(C.byref(pool), batch.n_seqs, m, hq, pages)
-    if n == 0:
-        raise ValueError(f"unsupported geometry B={batch.n_seqs} m={m} hq={hq} hkv={pool.hkv} d={pool.d} page={pool.page_size}")
+    key = (index, b, m, hq, pages, pshape, k_pages.dtype)
+    n = _attn_workspace.get(key)
+    if n is None:
+        n = lib.trb_attn_paged_workspace_bytes(pool, b, m, hq, pages)
+        if n == 0:
+            raise ValueError(f"unsupported geometry B={b} m={m} hq={hq} hkv={pshape[1]} d={d} page={pshape[2]}")
+        if len(_attn_workspace) > 4096:
+            _attn_workspace.clear()
+        _attn_workspace[key] = n
     # a fresh buffer for every call: calls on other streams and in other captured graphs never share one
-    ws = torch.empty(n, device=q.device, dtype=torch.uint8)
-    a = L.AttnPagedArgs(q.data_ptr(), out.data_ptr(), gate.data_ptr() if gate is not None else None, rs, hs, m, hq,
-                        pool.d ** -0.5 if scale is None else scale, pages, prefix_table.data_ptr() if pages else None, _cursor(prefix_len),
-                        ws.data_ptr(), n)
-    L.check(lib.trb_attn_paged(C.byref(pool), C.byref(batch), C.byref(a), torch._C._cuda_getCurrentRawStream(index)), "trb_attn_paged")
+    ws = q.new_empty((n // 2,))
+    a = _pack_attn(q.data_ptr(), out.data_ptr(), gp, rs, hs, m, hq, d ** -0.5 if scale is None else scale, pages, pt, *_length(prefix_len, index),
+                   ws.data_ptr(), n)
+    code = lib.trb_attn_paged(pool, batch, a, torch._C._cuda_getCurrentRawStream(index))
+    if code:
+        raise L.TrbError(code, "trb_attn_paged")
     return out
 
 
@@ -473,29 +512,33 @@ def spec_verify(probs, drafts, u, *, draft_probs=None, n_drafts=None, lens=None)
     advanced by what was accepted plus one.  Returns tokens [B, K + 1] int64 (accepted drafts, the new token, then -1) and
     n_accepted [B] int64, both on the device."""
     index = _on_device(probs, drafts, u, draft_probs, n_drafts, lens)
-    if probs.dim() != 3 or probs.dtype not in _PROB_TYPES or probs.stride(2) != 1:
+    shape, kind = probs.shape, _PROB_TYPES.get(probs.dtype)
+    ps, qs, qp, np_, lp, lw = probs.stride(), (0, 0), 0, 0, 0, 0
+    if len(shape) != 3 or kind is None or ps[2] != 1 or shape[1] < 1:
         raise ValueError("probs must be fp32, bf16 or fp16 [B, K + 1, V] with a contiguous last dim")
-    b, k, vocab = probs.shape[0], probs.shape[1] - 1, probs.shape[2]
-    if k < 0 or drafts.shape != (b, k) or drafts.dtype != torch.int64 or not drafts.is_contiguous():
+    b, k, vocab = shape[0], shape[1] - 1, shape[2]
+    if drafts.shape != (b, k) or drafts.dtype is not _I64 or not drafts.is_contiguous():
         raise ValueError("drafts must be contiguous int64 [B, K]")
-    if u.shape != (b, k + 1) or u.dtype != torch.float32 or not u.is_contiguous():
+    if u.shape != (b, k + 1) or u.dtype is not _F32 or not u.is_contiguous():
         raise ValueError("u must be contiguous float32 [B, K + 1]")
-    qs = (0, 0)
     if draft_probs is not None:
-        if draft_probs.shape != (b, k, vocab) or draft_probs.dtype != probs.dtype or draft_probs.stride(2) != 1:
+        qs, qp = draft_probs.stride(), draft_probs.data_ptr()
+        if draft_probs.shape != (b, k, vocab) or draft_probs.dtype is not probs.dtype or qs[2] != 1:
             raise ValueError("draft_probs must be [B, K, V] of the type of probs with a contiguous last dim")
-        qs = draft_probs.stride()
-    if n_drafts is not None and (n_drafts.shape != (b,) or n_drafts.dtype != torch.int32 or not n_drafts.is_contiguous()):
-        raise ValueError("n_drafts must be contiguous int32 [B]")
-    if lens is not None and (lens.shape != (b,) or lens.dtype not in (torch.int32, torch.int64) or not lens.is_contiguous()):
-        raise ValueError("lens must be contiguous int32 or int64 [B]")
-    tokens = torch.empty(b, k + 1, device=probs.device, dtype=torch.int64)
-    n = torch.empty(b, device=probs.device, dtype=torch.int64)
+    if n_drafts is not None:
+        if n_drafts.shape != (b,) or n_drafts.dtype is not _I32 or not n_drafts.is_contiguous():
+            raise ValueError("n_drafts must be contiguous int32 [B]")
+        np_ = n_drafts.data_ptr()
+    if lens is not None:
+        if lens.shape != (b,) or not (lens.dtype is _I64 or lens.dtype is _I32) or not lens.is_contiguous():
+            raise ValueError("lens must be contiguous int32 or int64 [B]")
+        lp, lw = lens.data_ptr(), 8 if lens.dtype is _I64 else 4
+    tokens, n = drafts.new_empty((b, k + 1)), drafts.new_empty((b,))
     if b == 0:
         return tokens, n
-    a = L.SpecVerifyArgs(probs.data_ptr(), draft_probs.data_ptr() if draft_probs is not None else None, probs.stride(0), probs.stride(1), qs[0], qs[1],
-                         drafts.data_ptr(), u.data_ptr(), n_drafts.data_ptr() if n_drafts is not None else None, tokens.data_ptr(), n.data_ptr(),
-                         lens.data_ptr() if lens is not None else None, lens.element_size() if lens is not None else 0, b, k, vocab,
-                         _PROB_TYPES[probs.dtype], 0)
-    L.check(L.lib().trb_spec_verify(C.byref(a), torch._C._cuda_getCurrentRawStream(index)), "trb_spec_verify")
+    a = _pack_verify(probs.data_ptr(), qp, ps[0], ps[1], qs[0], qs[1], drafts.data_ptr(), u.data_ptr(), np_, tokens.data_ptr(), n.data_ptr(), lp, lw, b, k,
+                     vocab, kind, 0)
+    code = L.lib().trb_spec_verify(a, torch._C._cuda_getCurrentRawStream(index))
+    if code:
+        raise L.TrbError(code, "trb_spec_verify")
     return tokens, n
