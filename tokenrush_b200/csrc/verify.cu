@@ -7,8 +7,9 @@
 // fp32 weights keeps its place next to a border).
 //
 // Bound by HBM: one row of p (and of q) per sequence.  One cluster of CTAs per sequence: each CTA sums its part of the
-// row warp by warp, the warps' totals go to every CTA of the cluster through distributed shared memory, and the one warp
-// whose range holds the border goes over its range (now in L2) once more to find the index.  No workspace, one launch.
+// row warp by warp, the warps' totals go to every CTA of the cluster through distributed shared memory, and the CTA
+// whose warp's part holds the border goes over that part (now in L2) once more, in eight pieces and then one of them step by step.  No
+// workspace, one launch.
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -90,11 +91,72 @@ __device__ __forceinline__ double sv_warp_sum(double x) {
     return x;
 }
 
+// This lane's share of the weights in [lo, hi).  Whole steps, four at a time: p' = max(p, 0) and q' = min(max(q, 0), p') clear
+// negative values and NaN, and p' - q' is the weight, exact enough in 64 bits; an infinity (which counts as zero) shows in the largest value seen, and
+// the steps are then done again one by one.  So are the ones that hold the index without weight.
+template <typename T, bool VEC>
+__device__ __forceinline__ double sv_sum(const SvRow<T> &r, int lo, int hi, int lane) {
+    constexpr int PER = SvStep<T, VEC>::PER, SPAN = SvStep<T, VEC>::SPAN, UNR = sizeof(T) == 2 && VEC ? 2 : 4;
+    double s0 = 0.0, s1 = 0.0;
+    int base = lo;
+    while (base < hi) {
+        if (base + UNR * SPAN <= hi && !(r.without >= base && r.without < base + UNR * SPAN)) {
+            T pv[UNR][PER], qv[UNR][PER];
+#pragma unroll
+            for (int x = 0; x < UNR; ++x) {
+                if constexpr (VEC) {
+                    *reinterpret_cast<uint4 *>(pv[x]) = *reinterpret_cast<const uint4 *>(r.p + base + x * SPAN + lane * PER);
+                    if (r.q) *reinterpret_cast<uint4 *>(qv[x]) = *reinterpret_cast<const uint4 *>(r.q + base + x * SPAN + lane * PER);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < PER; ++e) {
+                        pv[x][e] = r.p[base + x * SPAN + e * 32 + lane];
+                        if (r.q) qv[x][e] = r.q[base + x * SPAN + e * 32 + lane];
+                    }
+                }
+            }
+            double a0 = 0.0, a1 = 0.0;
+            float top = 0.f;
+#pragma unroll
+            for (int x = 0; x < UNR; ++x)
+#pragma unroll
+                for (int e = 0; e < PER; e += 2) {
+                    const float p0 = fmaxf(sv_to_float(pv[x][e]), 0.f), p1 = fmaxf(sv_to_float(pv[x][e + 1]), 0.f);
+                    double w0 = (double)p0, w1 = (double)p1;
+                    top = fmaxf(top, fmaxf(p0, p1));
+                    if (r.q) {
+                        const float q0 = fmaxf(sv_to_float(qv[x][e]), 0.f), q1 = fmaxf(sv_to_float(qv[x][e + 1]), 0.f);
+                        top = fmaxf(top, fmaxf(q0, q1));
+                        w0 -= (double)fminf(q0, p0);
+                        w1 -= (double)fminf(q1, p1);
+                    }
+                    a0 += w0;
+                    a1 += w1;
+                }
+            if (!__any_sync(0xffffffffu, !(top <= 3.402823466e38f))) {
+                s0 += a0;
+                s1 += a1;
+                base += UNR * SPAN;
+                continue;
+            }
+        }
+        const int end = min(hi, base + UNR * SPAN);
+        for (; base < end; base += SPAN) {
+            double w[PER];
+            sv_load<T, VEC>(r, base, hi, lane, w);
+#pragma unroll
+            for (int e = 0; e < PER; ++e) s0 += w[e];
+        }
+    }
+    return s0 + s1;
+}
+
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(SV_THREADS) spec_verify_kernel(const SpecVerifyParams a) {
     namespace cg = cooperative_groups;
     constexpr int PER = SvStep<T, VEC>::PER, SPAN = SvStep<T, VEC>::SPAN;
     __shared__ double sm_tot[2][SV_MAX_CLUSTER * SV_WARPS];             // totals of every warp of the cluster, in row order
+    __shared__ double sm_piece[SV_WARPS];
     __shared__ int sm_n;
     cg::cluster_group cluster = cg::this_cluster();
     const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
@@ -146,14 +208,7 @@ __global__ void __launch_bounds__(SV_THREADS) spec_verify_kernel(const SpecVerif
     cluster.barrier_wait();
     if (used) {
         for (int round = 0; round < 2; ++round) {                       // a second one only where the residual has no mass
-            double s = 0.0;
-            for (int base = lo; base < hi; base += SPAN) {
-                double w[PER];
-                sv_load<T, VEC>(row, base, hi, lane, w);
-#pragma unroll
-                for (int e = 0; e < PER; ++e) s += w[e];
-            }
-            s = sv_warp_sum(s);
+            const double s = sv_warp_sum(sv_sum<T, VEC>(row, lo, hi, lane));
             if (lane < ranks) *cluster.map_shared_rank(&sm_tot[round][part], lane) = s;
             cluster.sync();
             double own = 0.0;
@@ -192,13 +247,31 @@ __global__ void __launch_bounds__(SV_THREADS) spec_verify_kernel(const SpecVerif
         const int src = hits ? __ffs(hits) - 1 : 31 - __clz(with_mass); // none passes it: a number of 1 or more, or not a number
         const int at = __shfl_sync(0xffffffffu, hits ? hit : some, src);
         const double start = __shfl_sync(0xffffffffu, hits ? hit_start : some_start, src);
-        mine = at == part;
+        // the CTA that holds the part goes over it once more, first in eight pieces
+        if (at / SV_WARPS != rank) return;
+        const int a_lo = (int)((long long)at * steps / parts), a_n = (int)((long long)(at + 1) * steps / parts) - a_lo;
+        const int b_lo = (a_lo + warp * a_n / SV_WARPS) * SPAN, b_hi = min(a.vocab, (a_lo + (warp + 1) * a_n / SV_WARPS) * SPAN);
+        const double s = sv_warp_sum(sv_sum<T, VEC>(row, b_lo, b_hi, lane));
+        if (lane == 0) sm_piece[warp] = s;
+        __syncthreads();
+        double before = start, run = start;
+        int owner = -1, last_owner = 0;
+#pragma unroll
+        for (int x = 0; x < SV_WARPS; ++x) {
+            const double v = sm_piece[x];
+            if (v > 0.0) {
+                if (owner < 0 && before + v > border) { owner = x; run = before; }
+                if (owner < 0) { last_owner = x; some_start = before; }
+            }
+            before += v;
+        }
+        if (owner < 0) { owner = last_owner; run = some_start; }        // (sums in another order: the border lies behind the last piece with mass)
+        mine = owner == warp;
         if (mine) {
-            double run = start;
             int found = -1, last = -1;
-            for (int base = lo; base < hi && found < 0; base += SPAN) {
+            for (int base = b_lo; base < b_hi && found < 0; base += SPAN) {
                 double w[PER];
-                sv_load<T, VEC>(row, base, hi, lane, w);
+                sv_load<T, VEC>(row, base, b_hi, lane, w);
                 // running sums in index order: VEC lanes hold consecutive elements, else every 32 are a turn
                 constexpr int TURNS = VEC ? 1 : PER, EACH = VEC ? PER : 1;
 #pragma unroll
@@ -257,6 +330,17 @@ static cudaError_t launch_verify(const SpecVerifyParams &p, int n_seqs, int rank
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = pdl_enabled() ? 2 : 1;
+    if (ranks > 8) {                                                    // beyond the portable cluster size
+        static bool attr_set[64] = {};
+        int dev = 0;
+        cudaError_t e = cudaGetDevice(&dev);
+        if (e == cudaSuccess && !attr_set[dev & 63]) {
+            e = cudaFuncSetAttribute(spec_verify_kernel<T, true>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+            if (e == cudaSuccess) e = cudaFuncSetAttribute(spec_verify_kernel<T, false>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+            attr_set[dev & 63] = e == cudaSuccess;
+        }
+        if (e != cudaSuccess) return e;
+    }
     note_launch();
     return p.vec ? cudaLaunchKernelEx(&cfg, spec_verify_kernel<T, true>, p) : cudaLaunchKernelEx(&cfg, spec_verify_kernel<T, false>, p);
 }
@@ -282,7 +366,8 @@ extern "C" int trb_spec_verify(const trb_spec_verify_args_t *a, trb_stream_t str
     p.lens = a->lens; p.lens_width = a->lens_width; p.k = a->k; p.vocab = a->vocab;
     const int64_t strides = a->probs_seq_stride | a->probs_row_stride | (a->draft_probs ? a->draft_seq_stride | a->draft_row_stride : 0);
     p.vec = (((uintptr_t)a->probs | (uintptr_t)a->draft_probs) & 15) == 0 && (strides * size) % 16 == 0;
-    const int ranks = 8;
+    // one part of a row per warp of the cluster: 16 CTAs while that does not fill the SMs, 4 where a part would be less than a few steps
+    const int ranks = a->vocab <= 8192 ? 4 : a->n_seqs * 16 <= 2 * sm_count() ? 16 : 8;
     cudaStream_t st = (cudaStream_t)stream;
     pdl_forget(st);
     if (a->dtype == TRB_DT_F32) TRB_CUDA_CHECK(launch_verify<float>(p, a->n_seqs, ranks, st));
