@@ -6,11 +6,11 @@
 //
 // Bound by HBM bytes (every q, k, v element read once, written once) once the work per row is small, by latency for a handful of tokens.
 // Norm gain and rotation of a token are folded into two factors per dim, out = inv_rms (x A + partner(x) B), which a CTA computes once
-// per token in shared memory for all heads; a row then costs a warp one 16-byte load per lane, the sum of squares, one exchange with the
-// partner lanes (of bf16 pairs, before they are unpacked) and two packed multiply-adds per dim pair.  Issue slots are what the kernel
-// is short of next to HBM, so nothing is computed per row that a token or a head shares.
-// Many tokens: four per CTA and four heads per warp, the four tokens' rows of the next head requested while this head's are finished;
-// the chain sequence -> length -> page is then walked once for four tokens.  Few tokens: one, and one head per warp.
+// per token in shared memory for all heads.  Issue slots are what the kernel is short of next to HBM (a warp per row took 175
+// instructions a row and 66 us for 7472 tokens of 24 + 4 + 4 heads, 36 us at copy rate), so a row is held by D / 16 lanes, two
+// 16-byte chunks each, half a row apart: one stream of instructions serves 2 (256 dims) or 4 rows, sums take fewer exchanges, the upper half
+// of a row needs no partner when at most half the head is rotated, and a fully rotated head finds its partners in the same lane.
+// Many tokens: four per CTA, requested together; the chain sequence -> length -> page is then walked once for four.  Few tokens: one.
 // The angle is reduced to a fraction of a turn in 64 bits: at position 2e6 an fp32 product is already off by 0.1 rad.
 #include "paged.cuh"
 
@@ -39,35 +39,33 @@ __device__ __forceinline__ float div_by(float x, float b, float y) {
     return fmaf(fmaf(-q, b, x), y, q);
 }
 
-template <int N> __device__ __forceinline__ void load_bf16(const __nv_bfloat16 *src, uint32_t (&w)[N / 2]) {
-    if constexpr (N == 8) { const uint4 v = *reinterpret_cast<const uint4 *>(src); w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w; }
-    else { const uint2 v = *reinterpret_cast<const uint2 *>(src); w[0] = v.x; w[1] = v.y; }
-}
 __device__ __forceinline__ float2 unpack_bf16x2(uint32_t w) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
 
-template <int D, int TPC, int RPW>
+template <int D, int TPC, int R>
 __global__ void __launch_bounds__(PA_THREADS, 3) paged_append_kernel(const PagedAppendParams p) {
-    constexpr int EPT = D / 32, W = EPT / 2, F4 = EPT / 4;
-    __shared__ float4 sm_a[TPC][2][F4][32], sm_b[TPC][2][F4][32];        // factors of token, kind (q, k), piece of four dims, lane
+    constexpr int LPR = D / 16, RPI = 32 / LPR;                          // lanes of a row, rows (heads) of a warp
+    __shared__ float4 sm_a[TPC][3][4][LPR], sm_b[TPC][3][4][LPR];        // factors: token, kind (q, k, v), piece of four dims (chunk 0: 0, 1; chunk 1: 2, 3), lane
     __shared__ long long sm_own[TPC];                                    // own row, -1: the token writes no cache row
     __shared__ int sm_page[TPC];
-    const int t0 = blockIdx.x * TPC, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int t0 = blockIdx.x * TPC, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, l = lane % LPR;
     const int hq = p.q ? p.hq : 0, heads = hq + 2 * p.c.hkv;             // rows of a token: q heads, k heads, v heads
-    const int h0 = (blockIdx.y * PA_WARPS + warp) * RPW;
+    const int h0 = (blockIdx.y * PA_WARPS + warp) * R * RPI + lane / LPR;
     pdl_wait();
     pdl_launch_dependents();
 
-    uint32_t raw[TPC][W];
+    uint4 raw[TPC][2];
     auto request = [&](int h) {                                          // head h of the CTA's tokens
         const __nv_bfloat16 *src;
         long long step;
         if (h < hq) { src = p.q + h * p.qhs; step = p.qrs; }
         else if (h < hq + p.c.hkv) { src = p.k + (h - hq) * p.khs; step = p.krs; }
         else { src = p.v + (h - hq - p.c.hkv) * p.vhs; step = p.vrs; }
-        src += t0 * step + lane * EPT;
+        src += t0 * step + l * 8;
 #pragma unroll
         for (int tk = 0; tk < TPC; ++tk)
-            if (h < heads && t0 + tk < p.n_rows) load_bf16<EPT>(src + tk * step, raw[tk]);
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+                raw[tk][c] = h < heads && t0 + tk < p.n_rows ? *reinterpret_cast<const uint4 *>(src + tk * step + c * (D / 2)) : make_uint4(0u, 0u, 0u, 0u);
     };
     request(h0);
 
@@ -123,105 +121,141 @@ __global__ void __launch_bounds__(PA_THREADS, 3) paged_append_kernel(const Paged
             sn *= p.amplitude;
             if (!p.interleaved) { d = pair; e = pair + half; }
         }
-        const int at_d = d / EPT, at_e = e / EPT;                        // lane; then piece and place in it
-        const int f_d = d % EPT / 4, f_e = e % EPT / 4;
+        auto put = [&](int kind, int dim, float fa, float fb) {          // chunk dim / (D / 2) of lane dim % (D / 2) / 8
+            const int in = dim % (D / 2), piece = dim / (D / 2) * 2 + in % 8 / 4;
+            reinterpret_cast<float *>(&sm_a[tk][kind][piece][in / 8])[dim & 3] = fa;
+            reinterpret_cast<float *>(&sm_b[tk][kind][piece][in / 8])[dim & 3] = fb;
+        };
 #pragma unroll
-        for (int kind = 0; kind < 2; ++kind) {
-            const __nv_bfloat16 *w = kind ? p.kw : p.qw;
+        for (int kind = 0; kind < 3; ++kind) {
+            const __nv_bfloat16 *w = kind == 0 ? p.qw : kind == 1 ? p.kw : nullptr;
             const float gd = w ? 1.f + __bfloat162float(w[d]) : 1.f, ge = w ? 1.f + __bfloat162float(w[e]) : 1.f;
-            reinterpret_cast<float *>(&sm_a[tk][kind][f_d][at_d])[d & 3] = gd * cs;
-            reinterpret_cast<float *>(&sm_b[tk][kind][f_d][at_d])[d & 3] = -ge * sn;
-            reinterpret_cast<float *>(&sm_a[tk][kind][f_e][at_e])[e & 3] = ge * cs;
-            reinterpret_cast<float *>(&sm_b[tk][kind][f_e][at_e])[e & 3] = gd * sn;
+            const bool turn = kind < 2 && pair < half;                   // else -0: x * 1 + 0 * -0 is x, a negative zero too
+            put(kind, d, turn ? gd * cs : gd, turn ? -ge * sn : -0.f);
+            put(kind, e, turn ? ge * cs : ge, turn ? gd * sn : -0.f);
         }
     }
     __syncthreads();
 
-    // the lane that holds the partners of this one's dims (half layout: rd is a multiple of 2 EPT, so it is one lane for all of them)
-    const int hl = half / EPT;
-    const int partner = (lane < hl ? lane + hl : lane - hl) & 31;
+    // Where a chunk's partners are (half layout): chunk number x = c * LPR + l, partner x + hl or x - hl.  rd is a multiple of 16, so a chunk is
+    // rotated as a whole.
+    const int half8 = p.rd / 16, rot8 = 2 * half8;                       // chunks of half the rotation, of all of it
+    const int hl = half8;
+    const bool same_set = rot8 <= LPR, in_lane = hl == LPR;
 #pragma unroll 1
-    for (int r = 0; r < RPW; ++r) {
-        const int h_all = h0 + r;
-        if (h_all >= heads) break;
-        uint32_t now[TPC][W];
-#pragma unroll
-        for (int tk = 0; tk < TPC; ++tk)
-#pragma unroll
-            for (int e = 0; e < W; ++e) now[tk][e] = raw[tk][e];
-        if (r + 1 < RPW) request(h_all + 1);
-        const bool is_q = h_all < hq, is_v = h_all >= hq + p.c.hkv;
-        const int h = is_q ? h_all : is_v ? h_all - hq - p.c.hkv : h_all - hq;
-        const bool norm = (is_q ? p.qw : p.kw) != nullptr;
+    for (int r = 0; r < R; ++r) {
+        const int h_all = h0 + r * RPI;
+        if (h_all - lane / LPR >= heads) break;                          // (the same for the whole warp)
+        if (r > 0) request(h_all);
+        const bool ok = h_all < heads, is_q = h_all < hq, is_v = h_all >= hq + p.c.hkv;
+        const int h = is_q ? h_all : is_v ? h_all - hq - p.c.hkv : h_all - hq, kind = is_q ? 0 : is_v ? 2 : 1;
+        const bool norm = !is_v && (is_q ? p.qw : p.kw) != nullptr;
+        const bool any_norm = __any_sync(0xffffffffu, norm), any_rot = p.rd > 0 && __any_sync(0xffffffffu, !is_v);
+        const bool codes = !is_q && p.c.ks != nullptr, any_codes = __any_sync(0xffffffffu, codes && ok);
 #pragma unroll
         for (int tk = 0; tk < TPC; ++tk) {
             const int t = t0 + tk;
             if (t >= p.n_rows) break;
-            const int page = sm_page[tk];
-            float2 f[W];
+            const uint32_t x[8] = {raw[tk][0].x, raw[tk][0].y, raw[tk][0].z, raw[tk][0].w, raw[tk][1].x, raw[tk][1].y, raw[tk][1].z, raw[tk][1].w};
+            float2 f[8];
 #pragma unroll
-            for (int e = 0; e < W; ++e) f[e] = unpack_bf16x2(now[tk][e]);
-            if (!is_v) {
-                float inv = 1.f;
-                if (norm) {
-                    float2 ss = __fmul2_rn(f[0], f[0]);
+            for (int e = 0; e < 8; ++e) f[e] = unpack_bf16x2(x[e]);
+            float inv = 1.f;
+            if (any_norm) {
+                float2 ss = __fmul2_rn(f[0], f[0]);
 #pragma unroll
-                    for (int e = 1; e < W; ++e) ss = __ffma2_rn(f[e], f[e], ss);
-                    inv = rsqrtf(fmaf(warp_sum(ss.x + ss.y), 1.0f / D, p.eps));
-                }
-                uint32_t o[W];
+                for (int e = 1; e < 8; ++e) ss = __ffma2_rn(f[e], f[e], ss);
+                float s = ss.x + ss.y;
+#pragma unroll
+                for (int o = LPR / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+                inv = norm ? rsqrtf(fmaf(s, 1.0f / D, p.eps)) : 1.f;
+            }
+            // partners of the two chunks; zero where a dim has none (its factor is zero too, but zero times an infinity is not)
+            uint32_t o[8];
+            bool lower = any_rot, upper = any_rot && !(same_set && !p.interleaved);
+            if (p.interleaved) upper = any_rot && p.rd > D / 2;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) o[e] = 0u;
+            if (any_rot) {
                 if (p.interleaved) {
 #pragma unroll
-                    for (int e = 0; e < W; ++e) o[e] = lane * EPT + 2 * e < p.rd ? prmt(now[tk][e], 0, 0x1032) : 0u;
-                } else {
+                    for (int e = 0; e < 8; ++e) {
+                        const int dim = (e >> 2) * (D / 2) + l * 8 + (e & 3) * 2;
+                        o[e] = !is_v && dim < p.rd ? prmt(x[e], 0, 0x1032) : 0u;
+                    }
+                } else if (in_lane) {
 #pragma unroll
-                    for (int e = 0; e < W; ++e) {
-                        o[e] = __shfl_sync(0xffffffffu, now[tk][e], partner);
-                        o[e] = lane * EPT < p.rd ? o[e] : 0u;            // (another dim times zero would still carry an infinity)
+                    for (int e = 0; e < 8; ++e) o[e] = is_v ? 0u : x[e ^ 4];
+                } else if (same_set) {
+                    const int from = (lane & ~(LPR - 1)) + ((l < hl ? l + hl : l - hl) & (LPR - 1));
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        o[e] = __shfl_sync(0xffffffffu, x[e], from);
+                        o[e] = !is_v && l < rot8 ? o[e] : 0u;
+                    }
+                } else {                                                 // between half the head and all of it: a chunk's partner may be in either set
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        const int at = c * LPR + l, to = at < hl ? at + hl : at - hl;
+                        const int from = (lane & ~(LPR - 1)) + (to & (LPR - 1));
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const uint32_t a = __shfl_sync(0xffffffffu, x[e], from), b = __shfl_sync(0xffffffffu, x[4 + e], from);
+                            o[c * 4 + e] = is_v || at >= rot8 ? 0u : to < LPR ? a : b;
+                        }
                     }
                 }
-                const float2 inv2 = make_float2(inv, inv);
+            }
+            const float2 inv2 = make_float2(inv, inv);
 #pragma unroll
-                for (int x = 0; x < F4; ++x) {
-                    const float4 fa = sm_a[tk][is_q ? 0 : 1][x][lane], fb = sm_b[tk][is_q ? 0 : 1][x][lane];
-                    f[2 * x] = __fmul2_rn(__ffma2_rn(f[2 * x], make_float2(fa.x, fa.y), __fmul2_rn(unpack_bf16x2(o[2 * x]), make_float2(fb.x, fb.y))), inv2);
-                    f[2 * x + 1] = __fmul2_rn(__ffma2_rn(f[2 * x + 1], make_float2(fa.z, fa.w), __fmul2_rn(unpack_bf16x2(o[2 * x + 1]), make_float2(fb.z, fb.w))), inv2);
+            for (int y = 0; y < 4; ++y) {
+                const float4 fa = sm_a[tk][kind][y][l];
+                float2 u = make_float2(-0.f, -0.f), v = u;
+                if (y < 2 ? lower : upper) {
+                    const float4 fb = sm_b[tk][kind][y][l];
+                    u = __fmul2_rn(unpack_bf16x2(o[2 * y]), make_float2(fb.x, fb.y));
+                    v = __fmul2_rn(unpack_bf16x2(o[2 * y + 1]), make_float2(fb.z, fb.w));
+                }
+                f[2 * y] = __fmul2_rn(__ffma2_rn(f[2 * y], make_float2(fa.x, fa.y), u), inv2);
+                f[2 * y + 1] = __fmul2_rn(__ffma2_rn(f[2 * y + 1], make_float2(fa.z, fa.w), v), inv2);
+            }
+            const long long own = sm_own[tk];
+            const int page = sm_page[tk];
+            const long long row = (((long long)page * p.c.hkv + h) << p.c.page_shift) + (int)(own & ((1LL << p.c.page_shift) - 1));
+            if (ok && !codes && (is_q || page >= 0)) {
+                __nv_bfloat16 *dst = (is_q ? p.q_out + ((long long)t * p.hq + h) * D : (__nv_bfloat16 *)(is_v ? p.c.v : p.c.k) + row * D) + l * 8;
+                const bool zero = is_q && own < 0;
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    uint32_t ob[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) ob[e] = zero ? 0u : pack_bf16x2(f[c * 4 + e].x, f[c * 4 + e].y);
+                    *reinterpret_cast<uint4 *>(dst + c * (D / 2)) = make_uint4(ob[0], ob[1], ob[2], ob[3]);
                 }
             }
-            if (is_q || !p.c.ks) {
-                const bool zero = is_q && sm_own[tk] < 0;
-                uint32_t ob[W];
-#pragma unroll
-                for (int e = 0; e < W; ++e) ob[e] = zero ? 0u : pack_bf16x2(f[e].x, f[e].y);
-                __nv_bfloat16 *dst = nullptr;
-                if (is_q) dst = p.q_out + ((long long)t * p.hq + h) * D;
-                else if (page >= 0) {
-                    const int in_page = (int)(sm_own[tk] & ((1LL << p.c.page_shift) - 1));
-                    dst = (__nv_bfloat16 *)(is_v ? p.c.v : p.c.k) + ((((long long)page * p.c.hkv + h) << p.c.page_shift) + in_page) * D;
-                }
-                if (dst) {
-                    if constexpr (EPT == 8) *reinterpret_cast<uint4 *>(dst + lane * EPT) = make_uint4(ob[0], ob[1], ob[2], ob[3]);
-                    else *reinterpret_cast<uint2 *>(dst + lane * EPT) = make_uint2(ob[0], ob[1]);
-                }
-            } else if (page >= 0) {
-                const int in_page = (int)(sm_own[tk] & ((1LL << p.c.page_shift) - 1));
-                const long long row = (((long long)page * p.c.hkv + h) << p.c.page_shift) + in_page;
+            if (any_codes) {
                 float amax = 0.f;
 #pragma unroll
-                for (int e = 0; e < W; ++e) amax = fmaxf(amax, fmaxf(fabsf(f[e].x), fabsf(f[e].y)));
-                amax = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(amax)));       // not negative: ordered as their bits
-                const float sc = __fdiv_rn(fmaxf(amax, 1e-6f), 448.0f), rcp = __frcp_rn(sc);
-                uint32_t w[F4];
+                for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fmaxf(fabsf(f[e].x), fabsf(f[e].y)));
 #pragma unroll
-                for (int x = 0; x < F4; ++x) {
-                    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(div_by(f[2 * x].x, sc, rcp), div_by(f[2 * x].y, sc, rcp)), __NV_SATFINITE, __NV_E4M3);
-                    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(div_by(f[2 * x + 1].x, sc, rcp), div_by(f[2 * x + 1].y, sc, rcp)), __NV_SATFINITE, __NV_E4M3);
-                    w[x] = lo | hi << 16;
+                for (int s = LPR / 2; s > 0; s >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, s));
+                if (codes && ok && page >= 0) {
+                    const float sc = __fdiv_rn(fmaxf(amax, 1e-6f), 448.0f), rcp = __frcp_rn(sc);
+                    uint8_t *dst = (is_v ? p.c.v : p.c.k) + row * D + l * 8;
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        uint32_t w[2];
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const float2 a = f[c * 4 + 2 * e], b = f[c * 4 + 2 * e + 1];
+                            const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(div_by(a.x, sc, rcp), div_by(a.y, sc, rcp)), __NV_SATFINITE, __NV_E4M3);
+                            const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(div_by(b.x, sc, rcp), div_by(b.y, sc, rcp)), __NV_SATFINITE, __NV_E4M3);
+                            w[e] = lo | hi << 16;
+                        }
+                        *reinterpret_cast<uint2 *>(dst + c * (D / 2)) = make_uint2(w[0], w[1]);
+                    }
+                    if (l == 0) (is_v ? p.c.vs : p.c.ks)[row] = sc;
                 }
-                uint8_t *dst = (is_v ? p.c.v : p.c.k) + row * D + lane * EPT;
-                if constexpr (EPT == 8) *reinterpret_cast<uint2 *>(dst) = make_uint2(w[0], w[1]);
-                else *reinterpret_cast<uint32_t *>(dst) = w[0];
-                if (lane == 0) (is_v ? p.c.vs : p.c.ks)[row] = sc;
             }
         }
     }
@@ -240,7 +274,7 @@ extern "C" int trb_paged_append(const trb_paged_t *pool, const trb_batch_t *batc
     if (!a->cu && (a->rows_per_seq < 1 || (long long)a->rows_per_seq * batch->n_seqs != a->n_rows)) return TRB_E_ARG;
     if (a->rotary_dim < 0 || a->rotary_dim > pool->d || (a->rotary_dim & 1)) return TRB_E_UNSUPPORTED;
     if (a->rotary_dim > 0 && !a->inv_freq) return TRB_E_ARG;
-    if (a->rotary_dim > 0 && !a->interleaved && a->rotary_dim % (2 * (pool->d / 32))) return TRB_E_UNSUPPORTED;
+    if (a->rotary_dim > 0 && !a->interleaved && a->rotary_dim % 16) return TRB_E_UNSUPPORTED;
     const uintptr_t ptrs = (uintptr_t)a->q | (uintptr_t)a->k | (uintptr_t)a->v | (uintptr_t)a->q_out | (uintptr_t)a->q_norm_w | (uintptr_t)a->k_norm_w;
     const int64_t strides = (a->q ? a->q_row_stride | a->q_head_stride : 0) | a->k_row_stride | a->k_head_stride | a->v_row_stride | a->v_head_stride;
     if ((ptrs & 15) || (strides & 7) || ((uintptr_t)a->cu & 3) || ((uintptr_t)a->inv_freq & 7)) return TRB_E_ALIGN;
@@ -251,13 +285,14 @@ extern "C" int trb_paged_append(const trb_paged_t *pool, const trb_batch_t *batc
     p.n_rows = a->n_rows; p.rows_per_seq = a->rows_per_seq; p.hq = a->hq; p.rd = a->rotary_dim; p.interleaved = a->interleaved != 0;
     p.eps = a->eps; p.amplitude = a->amplitude; p.base = make_cursor(&a->base);
     const int heads = (a->q ? a->hq : 0) + 2 * p.c.hkv;
-    // four tokens per CTA and four heads per warp once that still gives every SM several CTAs
-    const bool many = (long long)(a->n_rows / 4) * ((heads + 31) / 32) >= 4LL * sm_count();
-    const int tpc = many ? 4 : 1, rows = PA_WARPS * (many ? 4 : 1);
+    // four tokens per CTA and two rounds of heads per warp once that still gives every SM several CTAs
+    const int rpi = 512 / pool->d;                                        // heads of a warp at a time
+    const bool many = (long long)(a->n_rows / 4) * ((heads + 16 * rpi - 1) / (16 * rpi)) >= 4LL * sm_count();
+    const int tpc = many ? 4 : 1, rows = PA_WARPS * rpi * (many ? 2 : 1);
     cudaStream_t st = (cudaStream_t)stream;
     pdl_forget(st);
-    TRB_CUDA_CHECK(launch_kernel(pool->d == 256 ? (many ? paged_append_kernel<256, 4, 4> : paged_append_kernel<256, 1, 1>)
-                                                : (many ? paged_append_kernel<128, 4, 4> : paged_append_kernel<128, 1, 1>),
+    TRB_CUDA_CHECK(launch_kernel(pool->d == 256 ? (many ? paged_append_kernel<256, 4, 2> : paged_append_kernel<256, 1, 1>)
+                                                : (many ? paged_append_kernel<128, 4, 2> : paged_append_kernel<128, 1, 1>),
                                  dim3((a->n_rows + tpc - 1) / tpc, (heads + rows - 1) / rows), dim3(PA_THREADS), 0, st, true, p));
     return TRB_OK;
 }
