@@ -29,7 +29,7 @@ __host__ inline int make_paged_view(const trb_paged_t *c, PagedView *o) {
     if (c->hkv > 64 || c->page_size < 16 || c->page_size > 65536 || (c->page_size & (c->page_size - 1))) return TRB_E_UNSUPPORTED;
     if (c->num_pages > 0x7fffffffLL / c->hkv) return TRB_E_UNSUPPORTED;
     if (((uintptr_t)c->k | (uintptr_t)c->v) & 15) return TRB_E_ALIGN;
-    if (((uintptr_t)c->k_scale | (uintptr_t)c->v_scale) & 3) return TRB_E_ALIGN;
+    if (((uintptr_t)c->k_scale | (uintptr_t)c->v_scale) & 15) return TRB_E_ALIGN;
     o->k = (uint8_t *)c->k; o->v = (uint8_t *)c->v;
     o->ks = c->kv_dtype == TRB_KV_FP8 ? c->k_scale : nullptr;
     o->vs = c->kv_dtype == TRB_KV_FP8 ? c->v_scale : nullptr;

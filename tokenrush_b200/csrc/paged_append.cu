@@ -54,18 +54,18 @@ __global__ void __launch_bounds__(PA_THREADS, 3) paged_append_kernel(const Paged
     pdl_launch_dependents();
 
     uint4 raw[TPC][2];
-    auto request = [&](int h) {                                          // head h of the CTA's tokens
-        const __nv_bfloat16 *src;
-        long long step;
-        if (h < hq) { src = p.q + h * p.qhs; step = p.qrs; }
-        else if (h < hq + p.c.hkv) { src = p.k + (h - hq) * p.khs; step = p.krs; }
-        else { src = p.v + (h - hq - p.c.hkv) * p.vhs; step = p.vrs; }
+    auto request = [&](int h) {                                          // head h of the CTA's tokens (beyond the last: the last, not stored)
+        h = min(h, heads - 1);
+        const bool of_q = h < hq, of_k = h < hq + p.c.hkv;
+        const __nv_bfloat16 *src = of_q ? p.q + h * p.qhs : of_k ? p.k + (h - hq) * p.khs : p.v + (h - hq - p.c.hkv) * p.vhs;
+        const long long step = of_q ? p.qrs : of_k ? p.krs : p.vrs;
         src += t0 * step + l * 8;
 #pragma unroll
-        for (int tk = 0; tk < TPC; ++tk)
+        for (int tk = 0; tk < TPC; ++tk) {
 #pragma unroll
-            for (int c = 0; c < 2; ++c)
-                raw[tk][c] = h < heads && t0 + tk < p.n_rows ? *reinterpret_cast<const uint4 *>(src + tk * step + c * (D / 2)) : make_uint4(0u, 0u, 0u, 0u);
+            for (int c = 0; c < 2; ++c) raw[tk][c] = *reinterpret_cast<const uint4 *>(src + c * (D / 2));
+            if (t0 + tk + 1 < p.n_rows) src += step;
+        }
     };
     request(h0);
 

@@ -7,20 +7,26 @@
 // takes an equal piece of it whatever the lengths are, and a piece that covers part of a sequence leaves a (max, sum,
 // acc) partial that paged_merge_kernel joins.  The lengths are device integers: every CTA finds its piece itself.
 //
-// Inside a CTA four warps work on key tiles of their own, with a private ring of stages filled by cp.async: no
-// barrier is passed while tiles stream.  A tile is 16 keys, so it lies in one page, and 16 rows of a page are
-// contiguous.  The products run with the keys (resp. the head dims) as the 16-row operand of mma.m16n8k16 and the
+// Inside a CTA four warps work on key tiles of their own, with a private ring of stages filled by TMA: no barrier is
+// passed while tiles stream.  A tile is 16 keys, so it lies in one page: a copy per 128-byte column, swizzled, and 64 bytes of scales.
+// The products run with the keys (resp. the head dims) as the 16-row operand of mma.m16n8k16 and the
 // query rows as the 8 columns, as in the contiguous decode kernel:
 //   S^T[16 keys x 8] = K Q^T,   O^T[dims x 8] += V^T P^T.
-// The order of dims inside a contraction is free, so a lane reads 16-byte chunks of a row (swizzled against bank
-// conflicts) instead of fragments, and the chunk's order is carried by how Q is laid out and O is read back.  e4m3 codes become f16 in
-// registers; the K scale multiplies the score, the V scale moves into the exponent, so codes are never scaled.
+// The order of dims inside a contraction is free, so a lane reads 16-byte chunks of a row instead of fragments, and the
+// chunk's order is carried by how Q is laid out and O is read back.  e4m3 codes become f16 in registers; the K scale
+// multiplies the score, the V scale moves into the exponent, so codes are never scaled.
+//
+// While tiles stream, three CTAs of four warps keep HBM full (a warp's 8 KB step takes 1.8 us).  What remains is what a sequence costs apart from
+// its tiles: finding its page, its query rows, the join of the warps.  The line therefore counts PS_TURN steps for the
+// start of every sequence, and the next sequence's first tiles and query rows are requested before the join of this one.
 #include "paged.cuh"
 #include "paged_prefix.cuh"
+#include "tmap.h"
 
 namespace trb {
 
-constexpr int PS_WARPS = 4, PS_THREADS = PS_WARPS * 32, PS_STAGES = 3;
+constexpr int PS_WARPS = 4, PS_THREADS = PS_WARPS * 32;
+constexpr int PS_TURN = 6;              // steps of four warps that a change of sequence costs
 
 struct PagedAttnParams {
     PagedView c;
@@ -44,11 +50,6 @@ struct PagedAttnParams {
     float *part_acc;                   // [hkv * groups][ctas + n_seqs][8 NS][D]
 };
 
-__device__ __forceinline__ void cp_async_16(uint32_t dst, const void *src, uint32_t src_bytes) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(src_bytes) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 __device__ __forceinline__ uint4 ld_shared_v4(uint32_t a) {
     uint4 v;
     asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
@@ -56,28 +57,41 @@ __device__ __forceinline__ uint4 ld_shared_v4(uint32_t a) {
 }
 
 template <int D_, bool FP8_, int NS_> struct ScanCfg {
-    static constexpr int D = D_, NS = NS_, SUB = D_ == 128 ? 2 : 1;     // 16-key tiles per pipeline step: 4 KB of K for e4m3, 8 KB for bf16
+    static constexpr int D = D_, NS = NS_, SUB = D_ == 128 && FP8_ ? 2 : 1;     // 16-key tiles per pipeline step: 8 KB of K and V, 16 KB for 256-dim bf16
     static constexpr bool FP8 = FP8_;
-    static constexpr int ROWB = D * (FP8 ? 1 : 2), CPR = ROWB / 16;    // bytes and 16-byte chunks of a row
+    static constexpr int ROWB = D * (FP8 ? 1 : 2), CPR = ROWB / 16, SEGS = ROWB / 128;   // bytes, 16-byte chunks and 128-byte columns of a row
     static constexpr int TILE = 16 * ROWB, STAGE = SUB * 2 * TILE;
-    static constexpr int SC = FP8 ? SUB * 128 : 0;                     // scales of a stage: 16 K, 16 V per tile
-    static constexpr int RING = PS_STAGES * (STAGE + SC);
+    static constexpr int STAGES = NS == 1 && STAGE == 8192 ? 2 : 3;
+    static constexpr int CTAS = STAGE > 8192 ? 1 : NS == 1 ? 3 : 2;    // per SM, by shared memory and registers
+    static constexpr int RING = STAGES * STAGE;                        // per warp
     static constexpr int KJ = CPR / 4, VC = CPR / 8;                   // chunks per lane of a K row, of a V row
     static constexpr int KS = D / 16;                                  // MMA steps of a QK product = row tiles of a PV product
-    static constexpr int OFF_Q = PS_WARPS * RING;                      // [NS][KS][32] uint2
+    static constexpr int RED = (NS * 8 * D * 4 + STAGE - 1) / STAGE;   // stages that a warp's accumulators take when they are exchanged
+    static constexpr int OFF_SC = PS_WARPS * RING;                     // [warps][stages][SUB][K, V][16] floats
+    static constexpr int OFF_Q = OFF_SC + (FP8 ? PS_WARPS * STAGES * SUB * 128 : 0);      // [NS][KS][32] uint2
     static constexpr int OFF_QINV = OFF_Q + (NS > 1 ? NS * KS * 256 : 0);      // [warps or slices][8] floats
-    static constexpr int OFF_ML = OFF_QINV + PS_WARPS * 32;                  // [warps][8 NS][2] floats
-    static constexpr int OFF_CNT = OFF_ML + PS_WARPS * NS * 64;        // [PG_MAX_SEQS + 1] ints, then 8 for the scan
-    static constexpr int SMEM = OFF_CNT + (PG_MAX_SEQS + 16) * 4;
-    static constexpr int RED = (NS * 8 * D * 4 + STAGE + SC - 1) / (STAGE + SC);   // stages that a warp's accumulators take when they are exchanged
-    static_assert(RED < PS_STAGES && NS <= PS_WARPS, "the exchange leaves a stage for the next sequence");
+    static constexpr int OFF_ML = OFF_QINV + PS_WARPS * 32;            // [warps][8 NS][2] floats
+    static constexpr int OFF_BAR = OFF_ML + PS_WARPS * NS * 64;        // [warps][4] mbarriers
+    static constexpr int OFF_CNT = OFF_BAR + PS_WARPS * 32;            // [PG_MAX_SEQS + 1] ints, then 8 for the scan
+    static constexpr int SMEM = OFF_CNT + (PG_MAX_SEQS + 16) * 4 + 1024;      // + slack to align the base
+    static_assert(RED < STAGES && NS <= PS_WARPS && STAGES <= 4, "the exchange leaves a stage for the next sequence");
+    static_assert(CTAS * (SMEM + 1024) <= 228 * 1024, "shared memory of an SM");
 };
 
+// Untiled copy global -> shared (both addresses and the size multiples of 16 bytes) that completes on the mbarrier.
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint64_t *bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(dst), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
+}
+
 template <typename C>
-__global__ void __launch_bounds__(PS_THREADS) paged_scan_kernel(const PagedAttnParams p) {
+__global__ void __launch_bounds__(PS_THREADS, C::CTAS)
+paged_scan_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const PagedAttnParams p) {
     constexpr int D = C::D, NS = C::NS, SUB = C::SUB, KS = C::KS, KJ = C::KJ, VC = C::VC, CPR = C::CPR;
+    constexpr int SEGS = C::SEGS, STAGES = C::STAGES;
     constexpr bool FP8 = C::FP8;
-    extern __shared__ __align__(128) uint8_t ps_smem[];
+    extern __shared__ uint8_t ps_smem_raw[];
+    uint8_t *ps_smem = ps_smem_raw + ((1024u - (smem_u32(ps_smem_raw) & 1023u)) & 1023u);
     float *sm_qinv = reinterpret_cast<float *>(ps_smem + C::OFF_QINV);
     float *sm_ml = reinterpret_cast<float *>(ps_smem + C::OFF_ML);
     int *sm_cnt = reinterpret_cast<int *>(ps_smem + C::OFF_CNT);
@@ -85,13 +99,22 @@ __global__ void __launch_bounds__(PS_THREADS) paged_scan_kernel(const PagedAttnP
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int j = blockIdx.y % p.c.hkv, grp = blockIdx.y / p.c.hkv, hg = blockIdx.y;
     const int rows = p.g * p.m, r0 = grp * 8 * NS;
-    const uint32_t ring = smem_u32(ps_smem + warp * C::RING);
+    const uint32_t ring = smem_u32(ps_smem + warp * C::RING), scales = smem_u32(ps_smem + C::OFF_SC) + warp * STAGES * SUB * 128;
+    uint64_t *full = reinterpret_cast<uint64_t *>(ps_smem + C::OFF_BAR) + warp * 4;      // one per stage
+    uint32_t phases = 0;                                               // bit s: parity of stage s's next completion
+    bool ok = true;                                                    // no wait of this warp has run out
+    if (lane == 0) {
+        for (int s = 0; s < STAGES; ++s) mbar_init(&full[s], 1u);
+        mbar_fence_init();
+        if (warp == 0) { tma_prefetch_desc(&tm_k); tma_prefetch_desc(&tm_v); }
+    }
+    __syncwarp();
     // behind the prefix kernel this one starts when that has passed its own wait: everything before both is complete, and what
     // the two write is apart.  It then waits at its end, so that its completion says the same of the prefix kernel.
     if (!p.after_prefix) pdl_wait();
     pdl_launch_dependents();
 
-    // ---- the line of pipeline steps: sm_cnt[b] = steps before sequence b
+    // ---- the line of pipeline steps: sequence b has places sm_cnt[b] .. sm_cnt[b + 1] - 1 of it, PS_TURN for its start and then its steps
     const bool report = blockIdx.x == 0 && blockIdx.y == 0;
     const int n_prefix = paged_prefix_rows(p.prefix_len, p.prefix_pages, p.c.page_shift, report && threadIdx.x == 0);
     const int prefix_tiles = (n_prefix + 15) >> 4;
@@ -101,7 +124,8 @@ __global__ void __launch_bounds__(PS_THREADS) paged_scan_kernel(const PagedAttnP
         int sum = 0;
         for (int b = b0; b < b0 + per && b < p.b.n_seqs; ++b) {
             const int own = paged_own_rows(p.b, b, p.m, p.c.page_shift, report);
-            const int steps = own < 0 ? 0 : (prefix_tiles + ((own + 15) >> 4) + SUB - 1) / SUB;
+            int steps = own < 0 ? 0 : (prefix_tiles + ((own + 15) >> 4) + SUB - 1) / SUB;
+            steps += steps > 0 ? PS_TURN : 0;
             sm_cnt[b] = sum;
             sum += steps;
         }
@@ -118,13 +142,13 @@ __global__ void __launch_bounds__(PS_THREADS) paged_scan_kernel(const PagedAttnP
         __syncthreads();
     }
     const int total = sm_cnt[p.b.n_seqs];
-    // a CTA gets at least one step for each of its warps
-    const int active = max(1, min(p.ctas, (total + PS_WARPS - 1) / PS_WARPS));
+    // a CTA gets about a step for each of its warps at least
+    const int active = max(1, min(p.ctas, total / PS_WARPS));
     if (report) {
         for (int b = threadIdx.x; b < p.b.n_seqs; b += PS_THREADS) {
             const int lo = sm_cnt[b], hi = sm_cnt[b + 1];
-            p.plan[2 * b] = hi > lo ? (int)((((long long)lo + 1) * active - 1) / total) : 0;      // the CTA that owns step lo
-            p.plan[2 * b + 1] = hi > lo ? (int)(((long long)hi * active - 1) / total) : -1;       // ... and step hi - 1
+            p.plan[2 * b] = hi > lo ? (int)((((long long)lo + PS_TURN + 1) * active - 1) / total) : 0;    // the CTA that has the first step
+            p.plan[2 * b + 1] = hi > lo ? (int)(((long long)hi * active - 1) / total) : -1;               // ... and the last
         }
     }
     if ((int)blockIdx.x >= active || total == 0) { pdl_wait(); return; }
@@ -155,77 +179,87 @@ __global__ void __launch_bounds__(PS_THREADS) paged_scan_kernel(const PagedAttnP
 #pragma unroll
         for (int sb = 0; sb < SUB; ++sb) pages[sb] = k < steps ? page_of((s0 + warp + k * PS_WARPS) * SUB + sb) : -1;
     };
+    // A step's copies, one per lane: K and V columns, K and V scales of each of its tiles.  A tile behind the sequence's last row, or of a
+    // page outside the pool, reads zeros (a coordinate outside the tensor).
     auto load_step = [&](int step, int stage, const int (&pg)[SUB]) {
-        const uint32_t base = ring + stage * (C::STAGE + C::SC);
+        constexpr int OPS = 2 * SEGS + (FP8 ? 2 : 0);
+        const int sb = SUB == 1 ? 0 : lane / OPS, op = lane - sb * OPS;
+        const int page = SUB == 1 || sb == 0 ? pg[0] : pg[SUB - 1];
+        const int x = step * SUB + sb - prefix_tiles, in_page = ((x < 0 ? x + prefix_tiles : x) * 16) & ((1 << p.c.page_shift) - 1);
+        if (lane == 0) {
+            int scaled = 0;
 #pragma unroll
-        for (int sb = 0; sb < SUB; ++sb) {
-            const int tile = step * SUB + sb, x = tile - prefix_tiles;
-            const int row = x < 0 ? tile * 16 : x * 16, limit = pg[sb] < 0 ? 0 : (x < 0 ? n_prefix : own);
-            const int left = limit - row;                              // rows of the tile that exist; the others are zero
-            const long long first = pg[sb] < 0 ? 0 : ((((long long)pg[sb] * p.c.hkv + j) << p.c.page_shift) + (row & ((1 << p.c.page_shift) - 1)));
-            const uint8_t *ks = p.c.k + first * C::ROWB + lane * 16, *vs = p.c.v + first * C::ROWB + lane * 16;
-            const uint32_t kd = base + sb * 2 * C::TILE, vd = kd + C::TILE;
-#pragma unroll
-            for (int i = 0; i < CPR / 2; ++i) {                        // 16 rows x CPR chunks over 32 lanes
-                const int idx = i * 32 + lane, r = idx / CPR, ch = idx % CPR;
-                const uint32_t n = r < left ? 16u : 0u;
-                const uint32_t off = r < left ? i * 512 : 0;
-                cp_async_16(kd + r * C::ROWB + ((ch ^ ((r & 1) << 2)) << 4), ks + off, n);
-                cp_async_16(vd + r * C::ROWB + ((ch ^ (r & 6)) << 4), vs + off, n);
-            }
-            if constexpr (FP8) {
-                const bool ok = (lane & 15) < left;
-                const float *sc = (lane < 16 ? p.c.ks : p.c.vs) + first + (ok ? (lane & 15) : 0);
-                asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(base + C::STAGE + sb * 128 + lane * 4), "l"(sc), "r"(ok ? 4u : 0u) : "memory");
+            for (int y = 0; y < SUB; ++y) scaled += pg[y] >= 0 ? 128 : 0;
+            mbar_arrive_expect_tx(&full[stage], C::STAGE + (FP8 ? scaled : 0));
+        }
+        __syncwarp();
+        if (lane < SUB * OPS) {
+            const bool of_v = op < 2 * SEGS ? op >= SEGS : op > 2 * SEGS;
+            if (op < 2 * SEGS) {
+                const int sg = of_v ? op - SEGS : op;
+                tma_load_4d(ps_smem + warp * C::RING + stage * C::STAGE + (sb * 2 + (of_v ? 1 : 0)) * C::TILE + sg * 2048, of_v ? &tm_v : &tm_k, &full[stage],
+                            0, sg, in_page, page < 0 ? -1 : page * p.c.hkv + j);
+            } else if (page >= 0) {
+                const long long row = (((long long)page * p.c.hkv + j) << p.c.page_shift) + in_page;
+                bulk_load(scales + (stage * SUB + sb) * 128 + (of_v ? 64 : 0), (of_v ? p.c.vs : p.c.ks) + row, 64u, &full[stage]);
             }
         }
-        cp_async_commit();
     };
-    // step k of a sequence goes to stage (k + RED) mod PS_STAGES: the first RED stages hold the accumulators that the warps
+    // step k of a sequence goes to stage (k + RED) mod STAGES: the first RED stages hold the accumulators that the warps
     // exchange at the end of the sequence before, while the first steps of this one are already on their way
-    constexpr int RED = C::RED, EARLY = PS_STAGES - RED;
+    constexpr int RED = C::RED, EARLY = STAGES - RED;
     auto request = [&](int k) {
         int now[SUB];
 #pragma unroll
         for (int sb = 0; sb < SUB; ++sb) now[sb] = pages[sb];
         fetch_pages(k + 1);
-        if (k < steps) load_step(s0 + warp + k * PS_WARPS, (k + RED) % PS_STAGES, now);
-        else cp_async_commit();
+        if (k < steps && ok) load_step(s0 + warp + k * PS_WARPS, (k + RED) % STAGES, now);
     };
-    auto begin = [&]() {                                               // sequence seq: its piece, and the first EARLY steps
-        s0 = max(lo, sm_cnt[seq]) - sm_cnt[seq];
-        s1 = min(hi, sm_cnt[seq + 1]) - sm_cnt[seq];
-        own = paged_own_rows(p.b, seq, p.m, p.c.page_shift, false);
-        len = load_len(p.b, seq);
-        own_table = p.b.table + seq * p.b.table_stride;
-        steps = s1 - s0 > warp ? (s1 - s0 - warp + PS_WARPS - 1) / PS_WARPS : 0;
-        fetch_pages(0);
-#pragma unroll
-        for (int k = 0; k < (EARLY < PS_STAGES - 1 ? EARLY : PS_STAGES - 1); ++k) request(k);
-    };
-    begin();
-    while (true) {
-        const int now = seq;
-#pragma unroll
-        for (int k = EARLY; k < PS_STAGES - 1; ++k) request(k);
-
-        // ---- the query rows as MMA fragments: step (jj, w) of lane (g, t) holds dims of chunk 4 jj + t.  e4m3: f16 with a power-of-two
-        // factor for each row (a bf16 value may lie outside f16's range); bf16: as they are.
-        constexpr int DPC = FP8 ? 16 : 8;                               // dims of a chunk
-        uint2 qf[KS];
-        float q_inv = 1.f;                                             // of row g of the slice
-        auto load_q = [&](int s) {
-            const int r = r0 + s * 8 + g;
-            const bool ok = r < rows;
-            const __nv_bfloat16 *src = p.q + (((long long)now * p.m + (ok ? r / p.g : 0)) * p.hq + j * p.g + (ok ? r % p.g : 0)) * D;
+    // ---- the query rows as MMA fragments: step (jj, w) of lane (g, t) holds dims of chunk 8 (jj / 2) + 2 t + jj % 2 (so that the eight lanes
+    // of a shared-memory phase, two rows by four t, meet eight different places of the swizzle).  e4m3: f16 with a power-of-two
+    // factor for each row (a bf16 value may lie outside f16's range); bf16: as they are.
+    constexpr int DPC = FP8 ? 16 : 8;                                  // dims of a chunk
+    uint2 qf[KS];
+    const int q_slice = NS == 1 ? 0 : warp, q_row = r0 + q_slice * 8 + g;      // one slice: every warp for itself; else a slice per warp
+    const bool q_ok = q_slice < NS && q_row < rows;
+    const long long q_at = ((long long)(q_ok ? q_row / p.g : 0) * p.hq + j * p.g + (q_ok ? q_row % p.g : 0)) * D;
+    auto begin = [&]() {                                               // sequence seq: its piece, its query rows and the first EARLY steps
+        const int first = sm_cnt[seq] + PS_TURN;
+        s0 = max(lo, first) - first;
+        s1 = min(hi, sm_cnt[seq + 1]) - first;
+        if (NS == 1 || warp < NS) {
+            const __nv_bfloat16 *src = p.q + (long long)seq * p.m * p.hq * D + q_at;
 #pragma unroll
             for (int jj = 0; jj < KJ; ++jj)
 #pragma unroll
                 for (int x = 0; x < DPC / 8; ++x) {
-                    const uint4 v = *reinterpret_cast<const uint4 *>(src + (4 * jj + t) * DPC + x * 8);
-                    qf[jj * (DPC / 4) + 2 * x] = ok ? make_uint2(v.x, v.y) : make_uint2(0u, 0u);
-                    qf[jj * (DPC / 4) + 2 * x + 1] = ok ? make_uint2(v.z, v.w) : make_uint2(0u, 0u);
+                    const uint4 v = *reinterpret_cast<const uint4 *>(src + (8 * (jj >> 1) + 2 * t + (jj & 1)) * DPC + x * 8);
+                    qf[jj * (DPC / 4) + 2 * x] = make_uint2(v.x, v.y);
+                    qf[jj * (DPC / 4) + 2 * x + 1] = make_uint2(v.z, v.w);
                 }
+        }
+        len = load_len(p.b, seq);
+        own = (int)min(len + p.m, (long long)p.b.table_pages << p.c.page_shift);
+        own_table = p.b.table + seq * p.b.table_stride;
+        steps = s1 - s0 > warp ? (s1 - s0 - warp + PS_WARPS - 1) / PS_WARPS : 0;
+        fetch_pages(0);
+#pragma unroll
+        for (int k = 0; k < (EARLY < STAGES - 1 ? EARLY : STAGES - 1); ++k) request(k);
+    };
+    if (lo >= sm_cnt[seq + 1] || hi <= sm_cnt[seq] + PS_TURN) {         // (the piece ends in the start of its only sequence)
+        pdl_wait();
+        return;
+    }
+    begin();
+    while (true) {
+        const int now = seq;
+#pragma unroll
+        for (int k = EARLY; k < STAGES - 1; ++k) request(k);
+
+        if (NS == 1 || warp < NS) {
+#pragma unroll
+            for (int x = 0; x < KS; ++x) qf[x] = q_ok ? qf[x] : make_uint2(0u, 0u);
+            float q_inv = 1.f;
             if constexpr (FP8) {
                 float amax = 0.f;
 #pragma unroll
@@ -247,20 +281,14 @@ __global__ void __launch_bounds__(PS_THREADS) paged_scan_kernel(const PagedAttnP
                     qf[x] = make_uint2(pack_f16x2(a.x * mult, a.y * mult), pack_f16x2(b.x * mult, b.y * mult));
                 }
             }
-        };
-        if constexpr (NS == 1) {
-            load_q(0);                                                 // every warp for itself, in registers
             if (t == 0) sm_qinv[warp * 8 + g] = q_inv;
-            __syncwarp();
-        } else {
-            if (warp < NS) {                                           // a slice per warp, through shared memory
-                load_q(warp);
+            if constexpr (NS > 1) {                                    // through shared memory
 #pragma unroll
                 for (int x = 0; x < KS; ++x) sm_q[(warp * KS + x) * 32 + lane] = qf[x];
-                if (t == 0) sm_qinv[warp * 8 + g] = q_inv;
             }
-            __syncthreads();
         }
+        if constexpr (NS > 1) __syncthreads();
+        else __syncwarp();
         // this thread's query rows are columns 2t, 2t + 1 of each slice
         float qinv[NS * 2], ref[NS * 2], l[NS * 2], acc[NS][KS][4];
         int last[NS * 2];                                              // own rows below this are visible
@@ -282,11 +310,24 @@ __global__ void __launch_bounds__(PS_THREADS) paged_scan_kernel(const PagedAttnP
                 for (int e = 0; e < 4; ++e) acc[s][a][e] = 0.f;
 
         for (int k = 0; k < steps; ++k) {
-            request(k + PS_STAGES - 1);
-            cp_async_wait<PS_STAGES - 1>();
-            __syncwarp();
-            const uint32_t base = ring + ((k + RED) % PS_STAGES) * (C::STAGE + C::SC);
-            const int step = s0 + warp + k * PS_WARPS;
+            request(k + STAGES - 1);
+            const int stage = (k + RED) % STAGES, step = s0 + warp + k * PS_WARPS;
+            ok = __all_sync(0xffffffffu, mbar_wait(&full[stage], (phases >> stage) & 1u));
+            if (!ok) steps = 0;                                        // (the output is undefined, but nothing hangs)
+            phases ^= 1u << stage;
+            const uint32_t base = ring + stage * C::STAGE;
+#pragma unroll
+            for (int sb = 0; sb < SUB; ++sb) {                         // V rows behind the last one: a weight of zero times NaN must not reach O
+                const int x = step * SUB + sb - prefix_tiles, left = x < 0 ? n_prefix - (x + prefix_tiles) * 16 : own - x * 16;
+                if (left < 16) {
+                    const int from = max(left, 0);
+                    for (int y = lane; y < (16 - from) * CPR; y += 32)
+                        *reinterpret_cast<uint4 *>(ps_smem + warp * C::RING + stage * C::STAGE + (sb * 2 + 1) * C::TILE + (y & 7) * 16 +
+                                                   (y >> 3) % SEGS * 2048 + (from + (y >> 3) / SEGS) * 128) = make_uint4(0u, 0u, 0u, 0u);
+                    fence_async_smem();
+                    __syncwarp();
+                }
+            }
 
             // S^T: two chains of MMAs per tile
             float sc[SUB][NS][4];
@@ -297,11 +338,11 @@ __global__ void __launch_bounds__(PS_THREADS) paged_scan_kernel(const PagedAttnP
                 for (int s = 0; s < NS; ++s)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) s2[s][0][e] = s2[s][1][e] = 0.f;
-                const uint32_t kb = base + sb * 2 * C::TILE + g * C::ROWB;
+                const uint32_t kb = base + sb * 2 * C::TILE + g * 128;
 #pragma unroll
                 for (int jj = 0; jj < KJ; ++jj) {
-                    const uint32_t ch = ((4 * jj + t) ^ ((g & 1) << 2)) << 4;
-                    const uint4 x = ld_shared_v4(kb + ch), y = ld_shared_v4(kb + 8 * C::ROWB + ch);
+                    const uint32_t ch = (jj >> 1) * 2048 + (((2 * t + (jj & 1)) ^ g) << 4);       // (rows g and g + 8 are swizzled alike)
+                    const uint4 x = ld_shared_v4(kb + ch), y = ld_shared_v4(kb + 8 * 128 + ch);
                     const uint32_t xw[4] = {x.x, x.y, x.z, x.w}, yw[4] = {y.x, y.y, y.z, y.w};
                     if constexpr (FP8) {
 #pragma unroll
@@ -341,8 +382,8 @@ __global__ void __launch_bounds__(PS_THREADS) paged_scan_kernel(const PagedAttnP
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         float kk, vv;
-                        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(kk) : "r"(base + C::STAGE + sb * 128 + (g + 8 * h) * 4));
-                        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(vv) : "r"(base + C::STAGE + sb * 128 + 64 + (g + 8 * h) * 4));
+                        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(kk) : "r"(scales + (stage * SUB + sb) * 128 + (g + 8 * h) * 4));
+                        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(vv) : "r"(scales + (stage * SUB + sb) * 128 + 64 + (g + 8 * h) * 4));
                         kf[h] = kk;
                         vl[h] = __log2f(vv);
                         vinv[sb][h] = __fdividef(1.f, vv);
@@ -353,12 +394,21 @@ __global__ void __launch_bounds__(PS_THREADS) paged_scan_kernel(const PagedAttnP
 #pragma unroll
                 for (int s = 0; s < NS; ++s)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float v = FP8 ? fmaf(sc[sb][s][e] * kf[e >> 1], qinv[s * 2 + (e & 1)], vl[e >> 1]) : sc[sb][s][e] * qinv[s * 2 + (e & 1)];
-                        const int limit = x < 0 ? n_prefix : last[s * 2 + (e & 1)];
-                        sc[sb][s][e] = row + g + 8 * (e >> 1) < limit ? v : -INFINITY;
-                        raise |= sc[sb][s][e] > ref[s * 2 + (e & 1)] + 8.f;
-                    }
+                    for (int e = 0; e < 4; ++e)
+                        sc[sb][s][e] = FP8 ? fmaf(sc[sb][s][e] * kf[e >> 1], qinv[s * 2 + (e & 1)], vl[e >> 1]) : sc[sb][s][e] * qinv[s * 2 + (e & 1)];
+                if (row + 16 > (x < 0 ? (long long)n_prefix : len + 1)) {      // a key of the tile is hidden from some row
+#pragma unroll
+                    for (int s = 0; s < NS; ++s)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int limit = x < 0 ? n_prefix : last[s * 2 + (e & 1)];
+                            if (row + g + 8 * (e >> 1) >= limit) sc[sb][s][e] = -INFINITY;
+                        }
+                }
+#pragma unroll
+                for (int s = 0; s < NS; ++s)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) raise |= sc[sb][s][e] > ref[s * 2 + (e & 1)] + 8.f;
             }
             // the reference of a row follows its maximum lazily: weights up to 2^8 fit f16, so it moves only when a score
             // passes it by more
@@ -410,12 +460,12 @@ __global__ void __launch_bounds__(PS_THREADS) paged_scan_kernel(const PagedAttnP
                         pb[s][h] = movmatrix_trans(pk);
                     }
                 }
-                const uint32_t vb = base + sb * 2 * C::TILE + C::TILE + 2 * t * C::ROWB;
+                const uint32_t vb = base + sb * 2 * C::TILE + C::TILE + 2 * t * 128;
 #pragma unroll
                 for (int c = 0; c < VC; ++c) {
-                    // keys 2t, 2t + 1, 2t + 8, 2t + 9: rows of equal (row & 6) = 2t & 6
-                    const uint32_t ch = ((g + 8 * c) ^ ((2 * t) & 6)) << 4;
-                    uint4 v[4] = {ld_shared_v4(vb + ch), ld_shared_v4(vb + C::ROWB + ch), ld_shared_v4(vb + 8 * C::ROWB + ch), ld_shared_v4(vb + 9 * C::ROWB + ch)};
+                    // keys 2t, 2t + 1, 2t + 8, 2t + 9
+                    const uint32_t c0 = c * 2048 + ((g ^ (2 * t)) << 4), c1 = c * 2048 + ((g ^ (2 * t + 1)) << 4);
+                    const uint4 v[4] = {ld_shared_v4(vb + c0), ld_shared_v4(vb + 128 + c1), ld_shared_v4(vb + 8 * 128 + c0), ld_shared_v4(vb + 9 * 128 + c1)};
 #pragma unroll
                     for (int w = 0; w < 4; ++w) {
                         const uint32_t k0 = w == 0 ? v[0].x : w == 1 ? v[0].y : w == 2 ? v[0].z : v[0].w;
@@ -443,7 +493,7 @@ __global__ void __launch_bounds__(PS_THREADS) paged_scan_kernel(const PagedAttnP
         }
         // every step of this sequence has been consumed: on to the next one that has some in this CTA's piece
         do ++seq; while (seq < p.b.n_seqs && sm_cnt[seq + 1] <= sm_cnt[seq]);
-        const bool more = seq < p.b.n_seqs && sm_cnt[seq] < hi;
+        const bool more = seq < p.b.n_seqs && sm_cnt[seq] + PS_TURN < hi;
         if (more) begin();
 
         // ---- join the four warps through their rings and write the piece's partial
@@ -496,9 +546,9 @@ __global__ void __launch_bounds__(PS_THREADS) paged_scan_kernel(const PagedAttnP
             }
         }
         if (!more) break;
+        fence_async_smem();                                            // (the exchange area is refilled by TMA)
         __syncthreads();
     }
-    cp_async_wait<0>();
     pdl_wait();
 }
 
@@ -607,7 +657,10 @@ static PagedAttnPlan paged_attn_plan(int d, bool fp8, int hkv, int hq, int n_seq
     const int rows = hq / hkv * m;
     o.ns = rows <= 8 ? 1 : 2;
     o.groups = (rows + 8 * o.ns - 1) / (8 * o.ns);
-    const int per_sm = fp8 ? 2 : 1;                                       // CTAs that fit an SM (shared memory)
+    const int per_sm = o.ns == 1 ? (d == 256 ? (fp8 ? ScanCfg<256, true, 1>::CTAS : ScanCfg<256, false, 1>::CTAS)
+                                             : (fp8 ? ScanCfg<128, true, 1>::CTAS : ScanCfg<128, false, 1>::CTAS))
+                                 : (d == 256 ? (fp8 ? ScanCfg<256, true, 2>::CTAS : ScanCfg<256, false, 2>::CTAS)
+                                             : (fp8 ? ScanCfg<128, true, 2>::CTAS : ScanCfg<128, false, 2>::CTAS));
     o.ctas = std::max(1, sm_count() * per_sm / (hkv * o.groups));
     o.splits = o.blocks = 0;
     if (prefix_rows > 0 && n_seqs > 1) {
@@ -653,13 +706,16 @@ static int launch_prefix(const PagedAttnParams &p, const PagedAttnPlan &plan, cu
 template <typename C>
 static int launch_scan(const PagedAttnParams &p, cudaStream_t st) {
     static bool attr_set[64] = {};
-    int dev = 0;
+    int dev = 0, rc;
     TRB_CUDA_CHECK(cudaGetDevice(&dev));
     if (!attr_set[dev & 63]) {
         TRB_CUDA_CHECK(cudaFuncSetAttribute(paged_scan_kernel<C>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
         attr_set[dev & 63] = true;
     }
-    TRB_CUDA_CHECK(launch_kernel(paged_scan_kernel<C>, dim3(p.ctas, p.c.hkv * p.groups), dim3(PS_THREADS), C::SMEM, st, true, p));
+    CUtensorMap mk, mv;
+    if ((rc = get_row_tile_map(p.c.k, 1 << p.c.page_shift, (int)(p.c.num_pages * p.c.hkv), C::ROWB, 16, &mk))) return rc;
+    if ((rc = get_row_tile_map(p.c.v, 1 << p.c.page_shift, (int)(p.c.num_pages * p.c.hkv), C::ROWB, 16, &mv))) return rc;
+    TRB_CUDA_CHECK(launch_kernel(paged_scan_kernel<C>, dim3(p.ctas, p.c.hkv * p.groups), dim3(PS_THREADS), C::SMEM, st, true, mk, mv, p));
     return TRB_OK;
 }
 
@@ -688,7 +744,7 @@ extern "C" int trb_attn_paged(const trb_paged_t *pool, const trb_batch_t *batch,
     if (a->prefix_pages > 0 && (rc = check_cursor(&a->prefix_len))) return rc;
     // rows are counted in 32 bits, with room for a step of tiles behind the last one
     if (((long long)a->prefix_pages + batch->table_pages) << p.c.page_shift > 0x7fffff00LL) return TRB_E_UNSUPPORTED;
-    if (((((long long)a->prefix_pages + batch->table_pages) << p.c.page_shift) / 16 + 2) * batch->n_seqs > 0x7fffffffLL) return TRB_E_UNSUPPORTED;
+    if (((((long long)a->prefix_pages + batch->table_pages) << p.c.page_shift) / 16 + 2 + PS_TURN) * batch->n_seqs > 0x7fffffffLL) return TRB_E_UNSUPPORTED;
     if ((((uintptr_t)a->q | (uintptr_t)a->out) & 15) || ((uintptr_t)a->workspace & 255) || ((uintptr_t)a->prefix_table & 3) || ((uintptr_t)a->gate & 1)) return TRB_E_ALIGN;
     const bool fp8 = p.c.ks != nullptr;
     const PagedAttnPlan plan = paged_attn_plan(pool->d, fp8, pool->hkv, a->hq, batch->n_seqs, a->m, (long long)a->prefix_pages << p.c.page_shift);
