@@ -7,7 +7,6 @@ from __future__ import annotations
 
 import ctypes as C
 import os
-import struct
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("TRB_KV_LIB") or os.path.join(HERE, "libtrb_kv.so")
@@ -88,23 +87,6 @@ class SpecVerifyArgs(C.Structure):
                 ("k", C.c_int32), ("vocab", C.c_int32), ("dtype", C.c_int32), ("reserved", C.c_int32)]
 
 
-def packer(cls):
-    """A function that lays out a structure's values (nested structures flattened, null pointers as 0) as bytes.  The batched
-    calls are made once per layer and step, and filling a ctypes structure field by field costs several times as much."""
-    codes = {C.c_void_p: "Q", C.c_int32: "i", C.c_int64: "q", C.c_float: "f", C.c_size_t: "Q"}
-
-    def walk(c):
-        out, at = "", 0
-        for name, t in c._fields_:
-            field = getattr(c, name)
-            out += "x" * (field.offset - at) + (walk(t) if issubclass(t, C.Structure) else codes[t])
-            at = field.offset + field.size
-        return out + "x" * (C.sizeof(c) - at)
-    form = struct.Struct("=" + walk(cls))
-    assert form.size == C.sizeof(cls)
-    return form.pack
-
-
 # symbol -> (restype, argtypes); every function include/trb_kv.h declares
 SIGNATURES = {
     "trb_version": (C.c_int, []),
@@ -132,11 +114,10 @@ SIGNATURES = {
                                   C.c_void_p, C.c_void_p]),
     "trb_attn_prefill": (C.c_int, [C.POINTER(Cache), C.c_void_p, C.c_void_p, C.c_int32, C.c_int32, C.c_int64, C.c_float,
                                    C.c_void_p]),
-    # (structures of these four: a pointer to one, or its bytes as packer() lays them out)
-    "trb_paged_append": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
-    "trb_attn_paged_workspace_bytes": (C.c_size_t, [C.c_void_p, C.c_int32, C.c_int32, C.c_int32, C.c_int32]),
-    "trb_attn_paged": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
-    "trb_spec_verify": (C.c_int, [C.c_void_p, C.c_void_p]),
+    "trb_paged_append": (C.c_int, [C.POINTER(Paged), C.POINTER(Batch), C.POINTER(PagedAppendArgs), C.c_void_p]),
+    "trb_attn_paged_workspace_bytes": (C.c_size_t, [C.POINTER(Paged), C.c_int32, C.c_int32, C.c_int32, C.c_int32]),
+    "trb_attn_paged": (C.c_int, [C.POINTER(Paged), C.POINTER(Batch), C.POINTER(AttnPagedArgs), C.c_void_p]),
+    "trb_spec_verify": (C.c_int, [C.POINTER(SpecVerifyArgs), C.c_void_p]),
     "trb_p2p_create": (C.c_int, [C.c_size_t, C.POINTER(C.c_void_p), C.c_void_p]),
     "trb_p2p_open": (C.c_int, [C.c_void_p, C.POINTER(C.c_void_p)]),
     "trb_p2p_close": (C.c_int, [C.c_void_p]),
@@ -162,6 +143,25 @@ def lib() -> C.CDLL:
             fn.restype, fn.argtypes = res, args
         _lib = handle
     return _lib
+
+
+_native = None
+
+
+def native():
+    """The native host side of the batched calls (csrc/binding.cpp), bound to the library's entry points."""
+    global _native
+    if _native is None:
+        handle = lib()
+        try:
+            from . import _binding
+        except ImportError as e:
+            raise ImportError(f"tokenrush_b200/_binding.so cannot be loaded ({e}): build it with `python -m tokenrush_b200.build`") from e
+        address = lambda f: C.cast(f, C.c_void_p).value          # noqa: E731
+        _binding.bind(address(handle.trb_paged_append), address(handle.trb_attn_paged_workspace_bytes), address(handle.trb_attn_paged),
+                      address(handle.trb_spec_verify), check)
+        _native = _binding
+    return _native
 
 
 def check(code: int, what: str):

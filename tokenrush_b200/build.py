@@ -5,9 +5,11 @@
 --timeline builds a second, diagnostic library (libtrb_kv_timeline.so) whose decode kernel records
 per-CTA time stamps; `bench.py --workload timeline` loads it.
 
-The library has no dependency on torch or Python; the host package loads it with ctypes.
+The library has no dependency on torch or Python; the host package loads it with ctypes.  The argument
+checks of the batched calls are native too (csrc/binding.cpp, built with the host compiler against torch).
 """
 import os
+import shutil
 import subprocess
 import sys
 
@@ -36,8 +38,32 @@ def up_to_date(lib: str = LIB) -> bool:
 LIB_TIMELINE = os.path.join(HERE, "libtrb_kv_timeline.so")
 
 
+BINDING = os.path.join(HERE, "_binding.so")
+
+
+def build_binding(force: bool = False) -> str:
+    src = os.path.join(CSRC, "binding.cpp")
+    deps = [src, os.path.join(HERE, "..", "include", "trb_kv.h")]
+    if not force and os.path.exists(BINDING) and all(os.path.getmtime(d) <= os.path.getmtime(BINDING) for d in deps):
+        return BINDING
+    import sysconfig
+    import torch
+    from torch.utils.cpp_extension import include_paths, library_paths
+    cuda = os.path.join(os.path.dirname(os.path.dirname(shutil.which(os.environ.get("NVCC", "nvcc")) or "/usr/local/cuda/bin/nvcc")), "include")
+    includes = include_paths() + [sysconfig.get_path("include"), cuda]
+    libs = [f for p in library_paths() for f in ("-L" + p, "-Wl,-rpath," + p)] + ["-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden", "-w",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"] + ["-I" + p for p in includes] + ["-o", BINDING, src] + libs
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        sys.stderr.write(r.stdout + r.stderr)
+        raise RuntimeError("the host compiler failed building _binding.so")
+    return BINDING
+
+
 def build(force: bool = False, verbose: bool = False, timeline: bool = False) -> str:
     lib = LIB_TIMELINE if timeline else LIB
+    build_binding(force)
     if not force and up_to_date(lib):
         return lib
     nvcc = os.environ.get("NVCC", "nvcc")

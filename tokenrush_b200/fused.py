@@ -334,61 +334,7 @@ def cursor_advance(pos_t, delta: int):
 
 # ------------------------------------------------------------------------------ batches over a paged cache
 
-_BF16, _F32, _F64, _I32, _I64, _E4M3 = torch.bfloat16, torch.float32, torch.float64, torch.int32, torch.int64, torch.float8_e4m3fn
-_pack_pool, _pack_batch, _pack_append = L.packer(L.Paged), L.packer(L.Batch), L.packer(L.PagedAppendArgs)
-_pack_attn, _pack_verify = L.packer(L.AttnPagedArgs), L.packer(L.SpecVerifyArgs)
-_attn_workspace: dict = {}           # geometry -> bytes
-
-
-def _on_device(first, *ts) -> int:
-    """The index of the current device, which all the tensors given have to be on."""
-    index = first.get_device()
-    for t in ts:
-        if t is not None and t.get_device() != index:
-            index = -1
-    if index < 0:
-        raise RuntimeError("tokenrush_b200 runs on CUDA tensors only (there is no CPU path), and on one device in a call")
-    if index != torch.cuda.current_device():
-        raise RuntimeError(f"the tensors are on cuda:{index}, the current device is cuda:{torch.cuda.current_device()}")
-    return index
-
-
-def _pool(k_pages, v_pages, k_scale, v_scale):
-    """One layer's pool of pages [PAGES, HKV, PAGE, D] (+ scales [PAGES, HKV, PAGE] for fp8): (trb_paged_t, its shape)."""
-    shape, kind = k_pages.shape, k_pages.dtype
-    if len(shape) != 4 or v_pages.shape != shape or not (k_pages.is_contiguous() and v_pages.is_contiguous()):
-        raise ValueError("pools must be contiguous [PAGES, HKV, PAGE, D] of one shape")
-    if v_pages.dtype is not kind or not (kind is _E4M3 or kind is _BF16):
-        raise TypeError("pools must be float8_e4m3fn or bfloat16")
-    pages, hkv, page, d = shape
-    if kind is _BF16:
-        return _pack_pool(k_pages.data_ptr(), v_pages.data_ptr(), 0, 0, hkv, d, L.TRB_KV_BF16, page, pages), shape
-    if (k_scale is None or v_scale is None or k_scale.dtype is not _F32 or v_scale.dtype is not _F32 or k_scale.shape != shape[:3]
-            or v_scale.shape != shape[:3] or not (k_scale.is_contiguous() and v_scale.is_contiguous())):
-        raise ValueError("an fp8 pool needs contiguous float32 k_scale and v_scale [PAGES, HKV, PAGE]")
-    return _pack_pool(k_pages.data_ptr(), v_pages.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), hkv, d, L.TRB_KV_FP8, page, pages), shape
-
-
-def _batch(table, lens):
-    """(trb_batch_t, number of sequences)"""
-    shape, stride, kind = table.shape, table.stride(), lens.dtype
-    if table.dtype is not _I32 or len(shape) != 2 or stride[1] != 1:
-        raise ValueError("table must be int32 [B, PAGES] with contiguous rows")
-    if not (kind is _I64 or kind is _I32) or lens.shape != shape[:1] or not lens.is_contiguous():
-        raise ValueError("lens must be contiguous int32 or int64 [B]")
-    return _pack_batch(table.data_ptr(), stride[0], lens.data_ptr(), 8 if kind is _I64 else 4, shape[0], shape[1], 0), shape[0]
-
-
-def _length(x, index):
-    """The fields of a trb_cursor_t: a python int, or a device tensor of one int32 / int64."""
-    if not isinstance(x, torch.Tensor):
-        return 0, 8, 0, int(x)
-    if not (x.dtype is _I64 or x.dtype is _I32) or x.numel() != 1:
-        raise TypeError("a length on the device is an int32 or int64 tensor of one element")
-    if x.get_device() != index:
-        raise RuntimeError("the length is not on the device of the other tensors")
-    return x.data_ptr(), 8 if x.dtype is _I64 else 4, 0, 0
-
+# (checked and called in native code, csrc/binding.cpp)
 
 def paged_append(k, v, k_pages, v_pages, table, lens, k_scale=None, v_scale=None, *, q=None, cu=None, base=0, q_norm_w=None, k_norm_w=None,
                  eps: float = 1e-6, inv_freq=None, interleaved: bool = False, amplitude: float = 1.0):
@@ -397,56 +343,11 @@ def paged_append(k, v, k_pages, v_pages, table, lens, k_scale=None, v_scale=None
     int32 stay on the device.  cu [B + 1] int32: first row of each sequence; None: T / B rows each.  Slots with lens[b] < 0
     and rows from cu[B] on are skipped.  On the way k (and q [T, HQ, D], if given) pass the heads' RMSNorm with
     the (1 + w) gain (where weights are given) and the rotation by (base + row) * inv_freq (float64 [rotary_dim / 2] from
-    `rope.frequencies`; base: an int or a device integer, the length of a shared prefix).  Pairs are (x, x + rotary_dim / 2) or,
-    interleaved, (2x, 2x + 1).  Returns the finished q [T, HQ, D] (None without q).  Two sequences of one call must not
-    share the pages they write."""
-    index = _on_device(k, v, k_pages, v_pages, k_scale, v_scale, table, lens, q, cu, q_norm_w, k_norm_w, inv_freq)
-    pool, shape = _pool(k_pages, v_pages, k_scale, v_scale)
-    batch, b = _batch(table, lens)
-    hkv, d, ks, vs = shape[1], shape[3], k.stride(), v.stride()
-    kshape = k.shape
-    t = kshape[0]
-    if kshape != (t, hkv, d) or v.shape != kshape:
-        raise ValueError("k and v must be [T, HKV, D] of the pool's heads")
-    if k.dtype is not _BF16 or v.dtype is not _BF16 or ks[2] != 1 or vs[2] != 1:
-        raise ValueError("k and v must be bfloat16 with a contiguous last dim")
-    out, qs, qp, op, hq = None, (0, 0), 0, 0, 0
-    if q is not None:
-        qshape, qs = q.shape, q.stride()
-        if len(qshape) != 3 or qshape[0] != t or qshape[2] != d or q.dtype is not _BF16 or qs[2] != 1:
-            raise ValueError("q must be bfloat16 [T, HQ, D] with a contiguous last dim")
-        hq = qshape[1]
-        out = q.new_empty(qshape)
-        qp, op = q.data_ptr(), out.data_ptr()
-    qw = kw = cup = rows = fp = rd = 0
-    if q_norm_w is not None:
-        if q_norm_w.dtype is not _BF16 or q_norm_w.shape != (d,) or not q_norm_w.is_contiguous():
-            raise ValueError("norm weights must be bfloat16 [D]")
-        qw = q_norm_w.data_ptr()
-    if k_norm_w is not None:
-        if k_norm_w.dtype is not _BF16 or k_norm_w.shape != (d,) or not k_norm_w.is_contiguous():
-            raise ValueError("norm weights must be bfloat16 [D]")
-        kw = k_norm_w.data_ptr()
-    if cu is None:
-        rows = t // b if b else 0
-        if rows * b != t:
-            raise ValueError("without cu every sequence has the same number of rows")
-    else:
-        if cu.dtype is not _I32 or cu.shape != (b + 1,) or not cu.is_contiguous():
-            raise ValueError("cu must be int32 [B + 1]")
-        cup = cu.data_ptr()
-    if inv_freq is not None:
-        if inv_freq.dtype is not _F64 or inv_freq.dim() != 1 or not inv_freq.is_contiguous():
-            raise ValueError("inv_freq must be float64 [rotary_dim / 2]")
-        fp, rd = inv_freq.data_ptr(), 2 * inv_freq.shape[0]
-    if t == 0:
-        return out
-    a = _pack_append(qp, k.data_ptr(), v.data_ptr(), op, qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], qw, kw, fp, cup, t, rows, hq, rd, 1 if interleaved else 0,
-                     eps, amplitude, *_length(base, index))
-    code = L.lib().trb_paged_append(pool, batch, a, torch._C._cuda_getCurrentRawStream(index))
-    if code:
-        raise L.TrbError(code, "trb_paged_append")
-    return out
+    `rope.frequencies`; base: an int or a device integer, the length of a shared prefix).  Pairs are (x, x + rotary_dim / 2)
+    (rotary_dim a multiple of 16) or, interleaved, (2x, 2x + 1).  Returns the finished q [T, HQ, D] (None without q).  Two
+    sequences of one call must not share the pages they write."""
+    return (L._native or L.native()).paged_append(k, v, k_pages, v_pages, table, lens, k_scale, v_scale, q, cu, base, q_norm_w, k_norm_w, eps, inv_freq,
+                                                  interleaved, amplitude)
 
 
 def attn_paged(q, k_pages, v_pages, table, lens, k_scale=None, v_scale=None, *, prefix_table=None, prefix_len=0, gate=None, scale=None, out=None):
@@ -455,52 +356,7 @@ def attn_paged(q, k_pages, v_pages, table, lens, k_scale=None, v_scale=None, *, 
     share (pages prefix_table [P] int32; prefix_len: an int or a device integer) and its own rows <= lens[b] + i.  Slots with
     lens[b] < 0 give zeros.  gate (optional): bf16 [B, M, HQ, D] view, out = bf16(o) * bf16(sigmoid(gate)) as in attn_decode_fused.
     Returns [B, M, HQ, D].  Lengths are read on the device, so a captured step serves all of them."""
-    index = _on_device(q, k_pages, v_pages, k_scale, v_scale, table, lens, prefix_table, gate, out)
-    pool, pshape = _pool(k_pages, v_pages, k_scale, v_scale)
-    batch, b = _batch(table, lens)
-    shape = q.shape
-    if len(shape) != 4 or shape[0] != b or shape[3] != pshape[3] or q.dtype is not _BF16 or not q.is_contiguous():
-        raise ValueError("q must be contiguous bf16 [B, M, HQ, D]")
-    m, hq, d, pages, pt = shape[1], shape[2], shape[3], 0, 0
-    if prefix_table is not None:
-        if prefix_table.dtype is not _I32 or prefix_table.dim() != 1 or not prefix_table.is_contiguous():
-            raise ValueError("prefix_table must be contiguous int32 [P]")
-        pages = prefix_table.shape[0]
-        if not isinstance(prefix_len, torch.Tensor) and not 0 <= prefix_len <= pages * pshape[2]:
-            raise ValueError("prefix_len exceeds the pages of prefix_table")
-        pt = prefix_table.data_ptr() if pages else 0
-    elif isinstance(prefix_len, torch.Tensor) or prefix_len != 0:
-        raise ValueError("a prefix needs its prefix_table")
-    rs = hs = gp = 0
-    if gate is not None:
-        if gate.shape != shape or gate.dtype is not _BF16 or gate.stride(3) != 1 or gate.stride(0) != m * gate.stride(1):
-            raise ValueError("gate must be a bf16 [B, M, HQ, D] view with equally spaced rows")
-        rs, hs, gp = gate.stride(1), gate.stride(2), gate.data_ptr()
-    if out is None:
-        out = q.new_empty(shape)
-    elif out.shape != shape or out.dtype is not _BF16 or not out.is_contiguous():
-        raise ValueError("out must be contiguous bf16 [B, M, HQ, D]")
-    lib = L.lib()
-    key = (index, b, m, hq, pages, pshape, k_pages.dtype)
-    n = _attn_workspace.get(key)
-    if n is None:
-        n = lib.trb_attn_paged_workspace_bytes(pool, b, m, hq, pages)
-        if n == 0:
-            raise ValueError(f"unsupported geometry B={b} m={m} hq={hq} hkv={pshape[1]} d={d} page={pshape[2]}")
-        if len(_attn_workspace) > 4096:
-            _attn_workspace.clear()
-        _attn_workspace[key] = n
-    # a fresh buffer for every call: calls on other streams and in other captured graphs never share one
-    ws = q.new_empty((n // 2,))
-    a = _pack_attn(q.data_ptr(), out.data_ptr(), gp, rs, hs, m, hq, d ** -0.5 if scale is None else scale, pages, pt, *_length(prefix_len, index),
-                   ws.data_ptr(), n)
-    code = lib.trb_attn_paged(pool, batch, a, torch._C._cuda_getCurrentRawStream(index))
-    if code:
-        raise L.TrbError(code, "trb_attn_paged")
-    return out
-
-
-_PROB_TYPES = {torch.float32: L.TRB_DT_F32, torch.bfloat16: L.TRB_DT_BF16, torch.float16: L.TRB_DT_F16}
+    return (L._native or L.native()).attn_paged(q, k_pages, v_pages, table, lens, k_scale, v_scale, prefix_table, prefix_len, gate, scale, out)
 
 
 def spec_verify(probs, drafts, u, *, draft_probs=None, n_drafts=None, lens=None):
@@ -511,34 +367,4 @@ def spec_verify(probs, drafts, u, *, draft_probs=None, n_drafts=None, lens=None)
     n_drafts [B] int32 (optional): drafts of each sequence, negative for an empty slot.  lens [B] (optional) is
     advanced by what was accepted plus one.  Returns tokens [B, K + 1] int64 (accepted drafts, the new token, then -1) and
     n_accepted [B] int64, both on the device."""
-    index = _on_device(probs, drafts, u, draft_probs, n_drafts, lens)
-    shape, kind = probs.shape, _PROB_TYPES.get(probs.dtype)
-    ps, qs, qp, np_, lp, lw = probs.stride(), (0, 0), 0, 0, 0, 0
-    if len(shape) != 3 or kind is None or ps[2] != 1 or shape[1] < 1:
-        raise ValueError("probs must be fp32, bf16 or fp16 [B, K + 1, V] with a contiguous last dim")
-    b, k, vocab = shape[0], shape[1] - 1, shape[2]
-    if drafts.shape != (b, k) or drafts.dtype is not _I64 or not drafts.is_contiguous():
-        raise ValueError("drafts must be contiguous int64 [B, K]")
-    if u.shape != (b, k + 1) or u.dtype is not _F32 or not u.is_contiguous():
-        raise ValueError("u must be contiguous float32 [B, K + 1]")
-    if draft_probs is not None:
-        qs, qp = draft_probs.stride(), draft_probs.data_ptr()
-        if draft_probs.shape != (b, k, vocab) or draft_probs.dtype is not probs.dtype or qs[2] != 1:
-            raise ValueError("draft_probs must be [B, K, V] of the type of probs with a contiguous last dim")
-    if n_drafts is not None:
-        if n_drafts.shape != (b,) or n_drafts.dtype is not _I32 or not n_drafts.is_contiguous():
-            raise ValueError("n_drafts must be contiguous int32 [B]")
-        np_ = n_drafts.data_ptr()
-    if lens is not None:
-        if lens.shape != (b,) or not (lens.dtype is _I64 or lens.dtype is _I32) or not lens.is_contiguous():
-            raise ValueError("lens must be contiguous int32 or int64 [B]")
-        lp, lw = lens.data_ptr(), 8 if lens.dtype is _I64 else 4
-    tokens, n = drafts.new_empty((b, k + 1)), drafts.new_empty((b,))
-    if b == 0:
-        return tokens, n
-    a = _pack_verify(probs.data_ptr(), qp, ps[0], ps[1], qs[0], qs[1], drafts.data_ptr(), u.data_ptr(), np_, tokens.data_ptr(), n.data_ptr(), lp, lw, b, k,
-                     vocab, kind, 0)
-    code = L.lib().trb_spec_verify(a, torch._C._cuda_getCurrentRawStream(index))
-    if code:
-        raise L.TrbError(code, "trb_spec_verify")
-    return tokens, n
+    return (L._native or L.native()).spec_verify(probs, drafts, u, draft_probs, n_drafts, lens)
