@@ -152,7 +152,7 @@ __device__ __forceinline__ double sv_sum(const SvRow<T> &r, int lo, int hi, int 
 }
 
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(SV_THREADS) spec_verify_kernel(const SpecVerifyParams a) {
+__global__ void __launch_bounds__(SV_THREADS, 3) spec_verify_kernel(const SpecVerifyParams a) {
     namespace cg = cooperative_groups;
     constexpr int PER = SvStep<T, VEC>::PER, SPAN = SvStep<T, VEC>::SPAN;
     __shared__ double sm_tot[2][SV_MAX_CLUSTER * SV_WARPS];             // totals of every warp of the cluster, in row order
@@ -203,8 +203,8 @@ __global__ void __launch_bounds__(SV_THREADS) spec_verify_kernel(const SpecVerif
     row.p = p0 + n * a.prs;
     row.q = fell && q0 ? q0 + n * a.qrs : nullptr;
     row.without = fell && !q0 ? drafts[n] : -1;
-    double total = 0.0, tot[SV_MAX_CLUSTER / 4], inc = 0.0;             // this lane's run of parts, and the sum up to its end
-    const int run_len = ranks / 4;                                      // parts per lane
+    double total = 0.0, tot[SV_MAX_CLUSTER / 4], inc = 0.0;             // this lane's run of parts, and the sum before it
+    const int run_len = (parts + 31) / 32;                              // parts per lane
     cluster.barrier_wait();
     if (used) {
         for (int round = 0; round < 2; ++round) {                       // a second one only where the residual has no mass
@@ -214,7 +214,7 @@ __global__ void __launch_bounds__(SV_THREADS) spec_verify_kernel(const SpecVerif
             double own = 0.0;
 #pragma unroll
             for (int e = 0; e < SV_MAX_CLUSTER / 4; ++e) {
-                tot[e] = e < run_len ? sm_tot[round][lane * run_len + e] : 0.0;
+                tot[e] = e < run_len && lane * run_len + e < parts ? sm_tot[round][lane * run_len + e] : 0.0;
                 own += tot[e];
             }
             inc = own;
@@ -366,8 +366,11 @@ extern "C" int trb_spec_verify(const trb_spec_verify_args_t *a, trb_stream_t str
     p.lens = a->lens; p.lens_width = a->lens_width; p.k = a->k; p.vocab = a->vocab;
     const int64_t strides = a->probs_seq_stride | a->probs_row_stride | (a->draft_probs ? a->draft_seq_stride | a->draft_row_stride : 0);
     p.vec = (((uintptr_t)a->probs | (uintptr_t)a->draft_probs) & 15) == 0 && (strides * size) % 16 == 0;
-    // one part of a row per warp of the cluster: 16 CTAs while that does not fill the SMs, 4 where a part would be less than a few steps
-    const int ranks = a->vocab <= 8192 ? 4 : a->n_seqs * 16 <= 2 * sm_count() ? 16 : 8;
+    // As many CTAs per row as let all rows run in one wave of three per SM, while a warp's part has a few steps.  (192 rows of
+    // 250000: 2 CTAs each; with 8, 3.5 waves paid the chain draft -> row -> sums -> border one after another.)  16 is the largest cluster.
+    const int steps = (a->vocab + 4096 / size - 1) / (4096 / size);       // (of 512 bytes, for the eight warps of a CTA)
+    int ranks = std::max(1, std::min(std::min(3 * sm_count() / a->n_seqs, 16), steps / 2));
+    if (ranks > 8 && ranks < 16) ranks = 8;                               // (beyond 8 only 16: the size the device is asked for)
     cudaStream_t st = (cudaStream_t)stream;
     pdl_forget(st);
     if (a->dtype == TRB_DT_F32) TRB_CUDA_CHECK(launch_verify<float>(p, a->n_seqs, ranks, st));
