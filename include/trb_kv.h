@@ -285,7 +285,7 @@ int trb_attn_prefill(const trb_cache_t *cache, const void *q, void *out, int32_t
  * One layer's pool: k, v [num_pages, hkv, page_size, d] contiguous, scales [num_pages, hkv, page_size]. */
 typedef struct trb_paged {
     void   *k, *v;
-    float  *k_scale, *v_scale;   /* NULL for a bf16 pool; positive and finite for live rows    */
+    float  *k_scale, *v_scale;   /* NULL for a bf16 pool; positive and finite for live rows; 16-byte aligned */
     int32_t hkv, d;              /* d in {128, 256}                                            */
     int32_t kv_dtype;            /* TRB_KV_BF16 or TRB_KV_FP8                                  */
     int32_t page_size;           /* rows per page: a power of two, 16 .. 65536                 */
@@ -293,7 +293,7 @@ typedef struct trb_paged {
 } trb_paged_t;
 
 /* The sequences of a step.  A page index outside the pool and a length beyond the table are recorded as
- * TRB_ST_CURSOR_RANGE; their rows are neither written nor read. */
+ * TRB_ST_CURSOR_RANGE: nothing is written there, and the attention output of such a sequence is undefined. */
 typedef struct trb_batch {
     const int32_t *table;        /* [n_seqs, table_pages], rows table_stride entries apart     */
     int64_t     table_stride;
@@ -308,7 +308,8 @@ typedef struct trb_batch {
  * (row t, head h, dim x) at t * row_stride + h * head_stride + x) is row t - cu[b] of sequence b (cu NULL: t = b *
  * rows_per_seq + i); it becomes own row lens[b] + i, position base + lens[b] + i.  q_norm_w / k_norm_w (optional):
  * RMSNorm of each head with the (1 + w) gain.  Rotation of the first rotary_dim dims by position * inv_freq[pair]
- * (computed in 64 bits), cos and sin times `amplitude`; pairs are (x, x + rotary_dim / 2) or, interleaved, (2x, 2x + 1).
+ * (computed in 64 bits), cos and sin times `amplitude`; pairs are (x, x + rotary_dim / 2), rotary_dim a multiple of 16, or,
+ * interleaved, (2x, 2x + 1), rotary_dim even.
  * Everything is held in fp32 and rounded once: q_out to bf16, K and V to bf16 or to e4m3 codes with the scale max(amax, 1e-6) / 448.
  * Rows at or beyond cu[n_seqs] and rows of empty slots write no cache row, and zeros to q_out. */
 typedef struct trb_paged_append_args {
@@ -341,6 +342,10 @@ typedef struct trb_attn_paged_args {
     void       *workspace;       /* trb_attn_paged_workspace_bytes() bytes, any contents        */
     size_t      workspace_bytes;
 } trb_attn_paged_args_t;
+/* The prefix is read by a kernel of its own when the scans of all sequences together would read at least min_bytes of it; a negative
+ * value restores the default (72 MB).  Both ways give results within the same tolerance; the switch exists for testing and
+ * measurement, and a workspace has to be sized under the setting it is used with. */
+int trb_set_paged_prefix_bytes(int64_t min_bytes);
 size_t trb_attn_paged_workspace_bytes(const trb_paged_t *pool, int32_t n_seqs, int32_t m, int32_t hq, int32_t prefix_pages);
 int trb_attn_paged(const trb_paged_t *pool, const trb_batch_t *batch, const trb_attn_paged_args_t *args, trb_stream_t stream);
 

@@ -262,9 +262,17 @@ def run_attention(tb, case, seed=5, peaked=False, gate=False, dev_prefix=False, 
     return call, q, lens, gt, (k, v, ks, vs, table)
 
 
+@pytest.fixture(params=[0, -1], ids=["prefix kernel", "scan"])
+def prefix_bytes(request, tb):
+    """A prefix read by its own kernel whatever its size, or (at these sizes) by the scan of every sequence."""
+    tb._lib.lib().trb_set_paged_prefix_bytes(request.param)
+    yield request.param
+    tb._lib.lib().trb_set_paged_prefix_bytes(-1)
+
+
 @pytest.mark.parametrize("case", ATTENDS)
 @pytest.mark.parametrize("peaked", [False, True])
-def test_attention(tb, case, peaked):
+def test_attention(tb, case, peaked, prefix_bytes):
     m, own, prefix, hq, hkv, d, fp8, page = case
     call, q, lens, _, (k, v, ks, vs, table) = run_attention(tb, case, peaked=peaked, dev_prefix=peaked, lens_t=torch.int32 if peaked else torch.int64)
     got = call()
@@ -280,7 +288,41 @@ def test_attention(tb, case, peaked):
     assert torch.equal(call(), got)                                      # the same again, bit for bit
 
 
-def test_attention_gate_and_out(tb):
+@pytest.mark.parametrize("hq,hkv,d,fp8", [(24, 4, 256, True), (24, 4, 256, False), (32, 8, 128, True), (16, 16, 128, False)])
+def test_attention_long(tb, hq, hkv, d, fp8):
+    """Hundreds of tiles per CTA, repeated (a wait that is missed shows as a timeout in the status word); 64 bits on the GPU."""
+    b, prefix, page, g = 30, 20011, 64, gen(9)
+    own = [1 + 173 * i % 2500 for i in range(b)]
+    table, pages = make_table(own + [prefix], page, 8)
+    k, v, ks, vs = make_pool(pages, hkv, page, d, fp8, 10)
+    q = torch.randn(b, 1, hq, d, device="cuda", generator=g).mul_(2).bfloat16()
+    own_table, pt = table[:b].cuda(), table[-1].cuda()
+    lens = torch.tensor(own, device="cuda") - 1
+    call = lambda: tb.fused.attn_paged(q, k, v, own_table, lens, ks, vs, prefix_table=pt, prefix_len=prefix)      # noqa: E731
+    got = call()
+    for _ in range(20):
+        assert torch.equal(call(), got)
+    assert tb._lib.device_status() == 0
+
+    def rows(x, s, t, n, j):
+        y = x[t[:-(-n // page)].long(), j].double() if not fp8 else x.view(torch.uint8)[t[:-(-n // page)].long(), j].view(x.dtype).double()
+        y = y if s is None else y * s[t[:-(-n // page)].long(), j].double().unsqueeze(-1)
+        return y.flatten(0, 1)[:n]
+    for j in range(0, hkv, max(1, hkv - 1)):
+        h = slice(j * hq // hkv, (j + 1) * hq // hkv)
+        kp, vp = rows(k, ks, pt, prefix, j), rows(v, vs, pt, prefix, j)
+        for i in range(0, b, 7):
+            kk, vv = torch.cat((kp, rows(k, ks, own_table[i], own[i], j))), torch.cat((vp, rows(v, vs, own_table[i], own[i], j)))
+            x = q[i, 0, h].double()
+            w = torch.softmax(x @ kk.T * d ** -0.5, 1)
+            o, a = w @ vv, w @ vv.abs()
+            e = d ** -0.5 * ((x.abs() @ kk.abs().T).amax(1, keepdim=True) * d * E32)
+            # as check_attention; e4m3 weights of the prefix kernel are off by at most 2^-18 of the row's largest weight where they are small
+            floor = 2.0 ** -18 * w.amax(1, keepdim=True) * vv.abs().sum(0) if fp8 else 0.0
+            assert ((got[i, 0, h].double() - o).abs() <= E16 * o.abs() + (E16 + 2 * e + 2.0 ** -20) * (a + o.abs()) * (1 + E16) + floor).all()
+
+
+def test_attention_gate_and_out(tb, prefix_bytes):
     case = (2, [40, 3], 70, 24, 4, 256, True, 64)
     call, q, lens, gt, _ = run_attention(tb, case, gate=True)
     plain = call()
@@ -291,7 +333,7 @@ def test_attention_gate_and_out(tb):
     assert ((out.float() - want).abs() <= (2 * E16 + E16 + 2.0 ** -16) * want.abs()).all()
 
 
-def test_attention_scale_and_large_values(tb):
+def test_attention_scale_and_large_values(tb, prefix_bytes):
     """q far outside f16's range, and a scale that brings the scores back."""
     case = (1, [33, 2], 20, 24, 4, 256, True, 16)
     call, q, lens, _, (k, v, ks, vs, table) = run_attention(tb, case)
@@ -300,7 +342,7 @@ def test_attention_scale_and_large_values(tb):
     assert torch.equal(call(scale=256 ** -0.5 * 2.0 ** -40), want)
 
 
-def test_attention_empty_rows(tb):
+def test_attention_empty_rows(tb, prefix_bytes):
     """No prefix rows and no own rows: zeros, whatever the pages hold."""
     case = (2, [2, 18], 0, 24, 4, 256, False, 16)
     call, q, lens, _, _ = run_attention(tb, case)
@@ -317,7 +359,7 @@ def test_attention_reports_lengths_beyond_the_table(tb):
     assert tb._lib.device_status() == tb._lib.ST_CURSOR_RANGE
 
 
-def test_captured_attention_follows_the_lengths(tb):
+def test_captured_attention_follows_the_lengths(tb, prefix_bytes):
     """One graph for all lengths, two graphs replayed on two streams at once, and the eager call beside them."""
     case = (2, [90, 300, 257], 400, 24, 4, 256, True, 64)
     call, q, lens, _, _ = run_attention(tb, case)
@@ -372,7 +414,7 @@ def test_refusals_on_the_gpu(tb):
 # ------------------------------------------------------------------------------ together
 
 @pytest.mark.parametrize("kv", ["fp8", "bf16"])
-def test_a_server_s_steps(tb, kv):
+def test_a_server_s_steps(tb, kv, prefix_bytes):
     """Shared prefix, prompts of unequal length, verify steps that advance the lengths on the device, a sequence that leaves and one that
     comes: attention after every step against 64-bit attention over the pool's rows."""
     cfg = tb.AttnConfig(n_attn=1)

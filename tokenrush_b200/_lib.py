@@ -115,6 +115,7 @@ SIGNATURES = {
     "trb_attn_prefill": (C.c_int, [C.POINTER(Cache), C.c_void_p, C.c_void_p, C.c_int32, C.c_int32, C.c_int64, C.c_float,
                                    C.c_void_p]),
     "trb_paged_append": (C.c_int, [C.POINTER(Paged), C.POINTER(Batch), C.POINTER(PagedAppendArgs), C.c_void_p]),
+    "trb_set_paged_prefix_bytes": (C.c_int, [C.c_int64]),
     "trb_attn_paged_workspace_bytes": (C.c_size_t, [C.POINTER(Paged), C.c_int32, C.c_int32, C.c_int32, C.c_int32]),
     "trb_attn_paged": (C.c_int, [C.POINTER(Paged), C.POINTER(Batch), C.POINTER(AttnPagedArgs), C.c_void_p]),
     "trb_spec_verify": (C.c_int, [C.POINTER(SpecVerifyArgs), C.c_void_p]),

@@ -646,6 +646,13 @@ __global__ void __launch_bounds__(256) paged_merge_kernel(const PagedAttnParams 
     else *reinterpret_cast<uint2 *>(dst) = *reinterpret_cast<const uint2 *>(ob);
 }
 
+// Bytes that the scans of all sequences would read of the prefix from which on it is read once, by a kernel of its own.  That kernel costs 8
+// to 12 us before it pays.  Measured with / without it (us; own rows 100 - 300): 24/4 heads x 256 e4m3, 8 sequences over 4096 rows (68 MB)
+// 23.4 / 20.6, 16 over 4096 (136 MB) 25.5 / 29.3, 32 over 16384 43 / 137; bf16 4 over 4096 (67 MB) 17.6 / 17.1, 8 over 4096 (134 MB) 19.5 / 25.2;
+// 32/8 x 128 e4m3, 8 over 4096 (69 MB) 19.8 / 20.7; 16/16 x 128 bf16, 8 over 1024 (67 MB) 16.0 / 16.1; 32 over 256 (33 MB) 24.7 / 17.8.
+constexpr long long PREFIX_BYTES = 72LL << 20;
+static std::atomic<long long> g_prefix_bytes{PREFIX_BYTES};
+
 // How a call is cut: query-row slices per CTA, row groups, CTAs per (kv head, group), pieces of the prefix and blocks of 128 query
 // rows of its kernel (0: the scan reads the prefix itself), and where the partials lie.
 struct PagedAttnPlan {
@@ -663,7 +670,8 @@ static PagedAttnPlan paged_attn_plan(int d, bool fp8, int hkv, int hq, int n_seq
                                              : (fp8 ? ScanCfg<128, true, 2>::CTAS : ScanCfg<128, false, 2>::CTAS));
     o.ctas = std::max(1, sm_count() * per_sm / (hkv * o.groups));
     o.splits = o.blocks = 0;
-    if (prefix_rows > 0 && n_seqs > 1) {
+    const double scanned = (double)n_seqs * o.groups * prefix_rows * hkv * (fp8 ? 2 * d + 8 : 4 * d);
+    if (prefix_rows > 0 && n_seqs > 1 && scanned >= (double)g_prefix_bytes) {
         const int tile = fp8 || d == 128 ? 128 : 64;
         const long long tiles = (prefix_rows + tile - 1) / tile;
         o.blocks = (int)(((long long)n_seqs * rows + 127) / 128);
@@ -729,6 +737,11 @@ static int check_paged_geometry(const trb_paged_t *pool, int n_seqs, int m, int 
     return TRB_OK;
 }
 
+extern "C" int trb_set_paged_prefix_bytes(int64_t min_bytes) {
+    g_prefix_bytes.store(min_bytes < 0 ? PREFIX_BYTES : min_bytes);
+    return TRB_OK;
+}
+
 extern "C" size_t trb_attn_paged_workspace_bytes(const trb_paged_t *pool, int32_t n_seqs, int32_t m, int32_t hq, int32_t prefix_pages) {
     PagedView v;
     if (make_paged_view(pool, &v) || check_paged_geometry(pool, n_seqs, m, hq, prefix_pages)) return 0;
@@ -771,11 +784,12 @@ extern "C" int trb_attn_paged(const trb_paged_t *pool, const trb_batch_t *batch,
     else rc = pool->d == 256 ? (fp8 ? launch_scan<ScanCfg<256, true, 2>>(p, st) : launch_scan<ScanCfg<256, false, 2>>(p, st))
                              : (fp8 ? launch_scan<ScanCfg<128, true, 2>>(p, st) : launch_scan<ScanCfg<128, false, 2>>(p, st));
     if (rc) return rc;
-    // few rows: their pieces are many, and eight warps share a row; many rows fill the SMs with a warp each
-    const long long out_rows = (long long)batch->n_seqs * a->m * a->hq;
-    const int wpr = out_rows <= 4LL * sm_count() ? 8 : 1;
-    const dim3 grid((unsigned)((out_rows * wpr + 7) / 8));
-    TRB_CUDA_CHECK(launch_kernel(pool->d == 256 ? (wpr == 8 ? paged_merge_kernel<256, 8> : paged_merge_kernel<256, 1>)
-                                                : (wpr == 8 ? paged_merge_kernel<128, 8> : paged_merge_kernel<128, 1>), grid, dim3(256), 0, st, true, p, plan.ns));
+    // as many warps per row as the SMs hold at once
+    const long long out_rows = (long long)batch->n_seqs * a->m * a->hq, most = 24LL * sm_count() / out_rows;
+    const int wpr = most >= 8 ? 8 : most >= 4 ? 4 : most >= 2 ? 2 : 1;
+    const bool wide = pool->d == 256;
+    auto *merge = wpr == 8 ? (wide ? paged_merge_kernel<256, 8> : paged_merge_kernel<128, 8>) : wpr == 4 ? (wide ? paged_merge_kernel<256, 4> : paged_merge_kernel<128, 4>)
+                  : wpr == 2 ? (wide ? paged_merge_kernel<256, 2> : paged_merge_kernel<128, 2>) : (wide ? paged_merge_kernel<256, 1> : paged_merge_kernel<128, 1>);
+    TRB_CUDA_CHECK(launch_kernel(merge, dim3((unsigned)((out_rows * wpr + 7) / 8)), dim3(256), 0, st, true, p, plan.ns));
     return TRB_OK;
 }

@@ -48,6 +48,10 @@ template <int D_, bool FP8_> struct PrefixCfg {
     static constexpr int OFF_MX = OFF_FAC + (FP8 ? SLOTS * 3 * BN * 4 : 0);   // [2][PX_WG][128] floats: row maxima of the four quarters
     static constexpr int OFF_BAR = OFF_MX + 2 * PX_WG * PX_BM * 4;
     static constexpr int SMEM = OFF_BAR + 256 + 1024;
+    // weights are staged as 2^(t - reference + LIFT).  The reference of a bf16 pool's row moves only when a score passes it by more than SLACK (a
+    // correction of O waits for the PV before it: 128 readers of 65536 rows 265 -> 245 us); e4m3 weights need the range for precision
+    // (hi + lo keep 8 bits down to 2^-10 of the row's largest weight and 2^-18 of it below; a slack of 3.75 would cost three bits of that and gains 2 %).
+    static constexpr float LIFT = FP8 ? 8.f : 0.f, SLACK = FP8 ? 0.f : 8.f;
     static constexpr int TM_S = 0, TM_O = 256, TM_Q = FP8 ? 0 : (D == 256 ? 128 : 384);
     static_assert(SMEM <= 227 * 1024, "shared memory budget");
     static_assert(STAGES * 2 * TILE >= PX_BM * D * 4, "the output block is turned in the ring");
@@ -66,9 +70,9 @@ paged_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
     uint64_t *bars = reinterpret_cast<uint64_t *>(smem + C::OFF_BAR);
     // K and V tiles have barriers of their own: a K tile is refilled as soon as its product has run
     uint64_t *k_full = bars, *v_full = k_full + STAGES, *k_free = v_full + STAGES, *v_free = k_free + STAGES;
-    uint64_t *s_full = v_free + STAGES, *p_full = s_full + 2, *o_done = p_full + 1, *o_last = o_done + 1, *q_ready = o_last + 1, *fac_full = q_ready + 1;
+    uint64_t *s_full = v_free + STAGES, *p_full = s_full + 2, *o_done = p_full + 2, *o_last = o_done + 1, *q_ready = o_last + 1, *fac_full = q_ready + 1;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(fac_full + SLOTS);
-    static_assert((4 * C::STAGES + 6 + C::SLOTS) * 8 + 4 <= 256, "barriers");
+    static_assert((4 * C::STAGES + 7 + C::SLOTS) * 8 + 4 <= 256, "barriers");
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int split = blockIdx.x % p.splits, blk = blockIdx.x / p.splits % p.blocks, j = blockIdx.x / p.splits / p.blocks;
@@ -81,9 +85,11 @@ paged_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
             mbar_init(&k_full[s], FP8 ? 33u : 1u); mbar_init(&v_full[s], 1u);      // e4m3: 32 lanes' scales come with the K tile
             mbar_init(&k_free[s], 1u); mbar_init(&v_free[s], 1u);
         }
-        for (int b = 0; b < 2; ++b) mbar_init(&s_full[b], 1u);
+        // P has a barrier per buffer: the softmax warps may finish tile i + 1 while the MMA warp still waits for V of tile i, and a second
+        // phase of one barrier would hide the first from its parity
+        for (int b = 0; b < 2; ++b) { mbar_init(&s_full[b], 1u); mbar_init(&p_full[b], PX_WARPS); }
         for (int b = 0; b < SLOTS; ++b) mbar_init(&fac_full[b], 1u);
-        mbar_init(p_full, PX_WARPS); mbar_init(o_done, 1u); mbar_init(o_last, 1u); mbar_init(q_ready, PX_WARPS);
+        mbar_init(o_done, 1u); mbar_init(o_last, 1u); mbar_init(q_ready, PX_WARPS);
         mbar_fence_init();
         tma_prefetch_desc(&tm_k); tma_prefetch_desc(&tm_v);
     }
@@ -225,7 +231,7 @@ paged_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
                 fence_async_smem();
                 __syncwarp();
             }
-            if (!(ok = mbar_wait(p_full, i & 1))) break;                           // P staged, O corrected
+            if (!(ok = mbar_wait(&p_full[i & 1], (i >> 1) & 1))) break;                           // P staged, O corrected
             tc_fence_after();
             if (lane == 0) {
                 if constexpr (FP8) {
@@ -364,9 +370,10 @@ paged_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
                 for (int c = 0; c < KPT / 2; ++c) mt4[c & 3] = pf_max3(mt4[c & 3], sv[2 * c], sv[2 * c + 1]);
                 mxbuf[part * PX_BM + row] = fmaxf(fmaxf(mt4[0], mt4[1]), fmaxf(mt4[2], mt4[3]));
                 named_barrier(1, PX_SOFTMAX);
-                const float m_new = fmaxf(pf_max3(m_run, mxbuf[row], mxbuf[PX_BM + row]), fmaxf(mxbuf[2 * PX_BM + row], mxbuf[3 * PX_BM + row]));
+                const float top = fmaxf(pf_max3(-INFINITY, mxbuf[row], mxbuf[PX_BM + row]), fmaxf(mxbuf[2 * PX_BM + row], mxbuf[3 * PX_BM + row]));
+                const float m_new = top > m_run + C::SLACK ? top : m_run;
                 const float m_safe = m_new == -INFINITY ? 0.f : m_new;
-                const float m_off = FP8 ? m_safe - 8.f : m_safe;                   // e4m3 weights are staged x 256
+                const float m_off = m_safe - C::LIFT;
                 const float alpha = m_new == -INFINITY ? 1.f : fast_exp2(m_run - m_safe);
                 // O is corrected only in warps where a row's maximum moved (S of this tile exists, so PV(i - 2) has completed: the
                 // parity cannot be mistaken)
@@ -428,7 +435,7 @@ paged_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
                 named_barrier(1, PX_SOFTMAX);
             }
             __syncwarp();
-            if (lane == 0) mbar_arrive(p_full);
+            if (lane == 0) mbar_arrive(&p_full[b]);
         }
         // ---- the piece's partial.  The last PV has a barrier of its own: a warp that skipped corrections does not know how many phases
         // of o_done have passed, so no parity of it would name the last one
@@ -453,9 +460,9 @@ paged_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
         }
         named_barrier(1, PX_SOFTMAX);
         const long long at = ((long long)split * p.c.hkv + j) * rows_all + q0;
-        if (row_ok && part == 0)                                                   // weights carry 2^8 with e4m3
+        if (row_ok && part == 0)
             *reinterpret_cast<float2 *>(p.part_ml + (at + row) * 2) =
-                make_float2(FP8 ? m_run - 8.f : m_run, (sm_l[row] + sm_l[PX_BM + row]) + (sm_l[2 * PX_BM + row] + sm_l[3 * PX_BM + row]));
+                make_float2(m_run - C::LIFT, (sm_l[row] + sm_l[PX_BM + row]) + (sm_l[2 * PX_BM + row] + sm_l[3 * PX_BM + row]));
         if (n_tiles > 0) {
             float4 *dst = reinterpret_cast<float4 *>(p.part_acc + at * D);
 #pragma unroll 4
