@@ -94,9 +94,12 @@ prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
     float *sm_mx = reinterpret_cast<float *>(smem + PF_OFF_MX);
     uint64_t *bars = reinterpret_cast<uint64_t *>(smem + PF_OFF_BAR);
     uint64_t *kv_full = bars, *kv_free = bars + 2 * PF_MAXST;   // [s]: K tile (+ scales) of stage s, [VB + s]: its V tile
-    uint64_t *s_full = bars + 4 * PF_MAXST, *p_full = s_full + 2, *o_done = s_full + 3, *q_ready = s_full + 4;
-    uint64_t *fac_full = s_full + 5;                            // [3]: the factor table of tile i (slot i mod 3) is written
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(s_full + 8);
+    // P has a barrier per buffer: the softmax warps may finish tile i+1 while the MMA warp still waits for V of tile i, and a
+    // second phase of one barrier would hide the first from its parity.  The last PV has one of its own (epilogue).
+    uint64_t *s_full = bars + 4 * PF_MAXST, *p_full = s_full + 2, *o_done = s_full + 4, *q_ready = s_full + 5, *o_last = s_full + 6;
+    uint64_t *fac_full = s_full + 7;                            // [3]: the factor table of tile i (slot i mod 3) is written
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(s_full + 10);
+    static_assert((4 * PF_MAXST + 10) * 8 + 4 <= 256, "barriers");
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int qb = blockIdx.x, h = blockIdx.y, j = h / p.g;
@@ -119,7 +122,8 @@ prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
         }
         for (int b = 0; b < 2; ++b) mbar_init(&s_full[b], 1u);
         for (int b = 0; b < 3; ++b) mbar_init(&fac_full[b], 1u);
-        mbar_init(p_full, 8u); mbar_init(o_done, 1u); mbar_init(q_ready, 8u);
+        for (int b = 0; b < 2; ++b) mbar_init(&p_full[b], 8u);
+        mbar_init(o_done, 1u); mbar_init(o_last, 1u); mbar_init(q_ready, 8u);
         mbar_fence_init();
         tma_prefetch_desc(&tm_k); tma_prefetch_desc(&tm_v);
     }
@@ -242,7 +246,7 @@ prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
             PF_TL(i, 12);
             if (!(ok = mbar_wait(&kv_full[VB + s], (i / STAGES) & 1))) break;      // V tile landed
             PF_TL(i, 13);
-            if (!(ok = mbar_wait(p_full, i & 1))) break;                        // P of tile i staged (and O corrected)
+            if (!(ok = mbar_wait(&p_full[i & 1], (i >> 1) & 1))) break;         // P of tile i staged (and O corrected)
             PF_TL(i, 14);
             tc_fence_after();
             if (lane == 0) {
@@ -264,7 +268,7 @@ prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
                     }
                 }
                 tc_commit(&kv_free[VB + s]);
-                tc_commit(o_done);
+                tc_commit(i == n_tiles - 1 ? o_last : o_done);
             }
             PF_TL(i, 15);
             __syncwarp();
@@ -447,14 +451,12 @@ prefill_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__
             tmem_st_wait();
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(p_full);
+            if (lane == 0) mbar_arrive(&p_full[b]);
             PF_TL(i, 7);
         }
         // ---- epilogue: O / l -> bf16 (with e4m3 both carry the factor 256); l = sum of the two halves' partial sums
-        // (a warp that skipped corrections may be two PVs behind the barrier's phase: one step at a time,
-        // so that a parity always names the phase it is meant for)
-        if (ok && n_tiles > 1) ok = mbar_wait(o_done, (n_tiles - 2) & 1);
-        if (ok && n_tiles > 0) ok = mbar_wait(o_done, (n_tiles - 1) & 1);
+        // (a warp that skipped corrections does not know how many phases of o_done have passed: no parity of it would name the last one)
+        if (ok && n_tiles > 0) ok = mbar_wait(o_last, 0);
         tc_fence_after();
         sm_mx[half * PF_BM + row] = l_run;
         named_barrier(1, PF_SOFTMAX_THREADS);
