@@ -359,6 +359,43 @@ def test_attention_reports_lengths_beyond_the_table(tb):
     assert tb._lib.device_status() == tb._lib.ST_CURSOR_RANGE
 
 
+def test_absurd_lengths_read_and_write_nothing_outside(tb, prefix_bytes):
+    case = (2, [16, 32, 20], 40, 24, 4, 256, True, 16)
+    call, q, lens, _, (k, v, ks, vs, table) = run_attention(tb, case)
+    kp, vp = (rows_of(y, z, table[-1], 40, 16) for y, z in ((k, ks), (v, vs)))
+    k0 = k.clone()
+    x = torch.zeros(6, 4, 256, device="cuda", dtype=torch.bfloat16)
+    for n in (2 ** 63 - 1, 2 ** 62, 2 ** 31, 2 ** 31 - 1, -2 ** 63):
+        lens[1] = n
+        got = call()
+        assert tb._lib.device_status() == (0 if n < 0 else tb._lib.ST_CURSOR_RANGE)
+        for i, own in ((0, 16), (2, 20)):                                # (not the same bits: the cut of the line depends on every length)
+            check_attention(got[i], q[i].double().cpu(), kp, vp, *(rows_of(y, z, table[i], own, 16) for y, z in ((k, ks), (v, vs))), 256 ** -0.5, (n, i))
+        others = lens.clone()
+        others[0] = others[2] = -1
+        tb.fused.paged_append(x, x, k, v, table[:3].cuda(), others, ks, vs)
+        tb._lib.device_status()
+        assert torch.equal(k.view(torch.uint8), k0.view(torch.uint8))
+
+
+def test_on_another_stream(tb, prefix_bytes):
+    """Calls run on the current stream: their inputs are made there and their outputs are ready there."""
+    case = (1, [300, 20, 64], 200, 24, 4, 256, False, 32)
+    call, q, lens, _, _ = run_attention(tb, case)
+    want = call()
+    torch.cuda.synchronize()
+    q0 = q.clone()
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        for _ in range(5):
+            q.zero_()
+            torch.cuda._sleep(200000)
+            q.copy_(q0)
+            got = call() + 0
+    s.synchronize()
+    assert torch.equal(got, want)
+
+
 def test_captured_attention_follows_the_lengths(tb, prefix_bytes):
     """One graph for all lengths, two graphs replayed on two streams at once, and the eager call beside them."""
     case = (2, [90, 300, 257], 400, 24, 4, 256, True, 64)

@@ -67,7 +67,7 @@ __device__ __forceinline__ int paged_own_rows(const BatchView &b, int seq, int m
     const long long len = load_len(b, seq);
     if (len < 0) return -1;                                            // an empty slot
     const long long most = (long long)b.table_pages << page_shift;
-    if (len + m > most) {
+    if (len > most - m) {                                              // (no sum: a length may be anything)
         if (report) raise_status(TRB_ST_CURSOR_RANGE);
         return (int)most;
     }

@@ -239,9 +239,9 @@ paged_scan_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
                 }
         }
         len = load_len(p.b, seq);
-        own = (int)min(len + p.m, (long long)p.b.table_pages << p.c.page_shift);
+        own = (int)(min(len, ((long long)p.b.table_pages << p.c.page_shift) - p.m) + p.m);
         own_table = p.b.table + seq * p.b.table_stride;
-        steps = s1 - s0 > warp ? (s1 - s0 - warp + PS_WARPS - 1) / PS_WARPS : 0;
+        steps = ok && s1 - s0 > warp ? (s1 - s0 - warp + PS_WARPS - 1) / PS_WARPS : 0;
         fetch_pages(0);
 #pragma unroll
         for (int k = 0; k < (EARLY < STAGES - 1 ? EARLY : STAGES - 1); ++k) request(k);
