@@ -10,13 +10,15 @@
 // instructions a row and 66 us for 7472 tokens of 24 + 4 + 4 heads, 36 us at copy rate), so a row is held by D / 16 lanes, two
 // 16-byte chunks each, half a row apart: one stream of instructions serves 2 (256 dims) or 4 rows, sums take fewer exchanges, the upper half
 // of a row needs no partner when at most half the head is rotated, and a fully rotated head finds its partners in the same lane.
-// Many tokens: four per CTA, requested together; the chain sequence -> length -> page is then walked once for four.  Few tokens: one.
+// Before its first row a CTA walks a chain of latencies (sequence -> length -> page, angles, factors), so many small ones are resident: two tokens
+// and four warps each, eight CTAs per SM (with four tokens and eight warps, three per SM, 7472 tokens took 59 us, now 51).  Few tokens: one per CTA, one
+// round of heads.
 // The angle is reduced to a fraction of a turn in 64 bits: at position 2e6 an fp32 product is already off by 0.1 rad.
 #include "paged.cuh"
 
 namespace trb {
 
-constexpr int PA_THREADS = 256, PA_WARPS = PA_THREADS / 32;
+constexpr int PA_THREADS = 128, PA_WARPS = PA_THREADS / 32;
 
 struct PagedAppendParams {
     PagedView c;
@@ -42,7 +44,7 @@ __device__ __forceinline__ float div_by(float x, float b, float y) {
 __device__ __forceinline__ float2 unpack_bf16x2(uint32_t w) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
 
 template <int D, int TPC, int R>
-__global__ void __launch_bounds__(PA_THREADS, 3) paged_append_kernel(const PagedAppendParams p) {
+__global__ void __launch_bounds__(PA_THREADS, 8) paged_append_kernel(const PagedAppendParams p) {
     constexpr int LPR = D / 16, RPI = 32 / LPR;                          // lanes of a row, rows (heads) of a warp
     __shared__ float4 sm_a[TPC][3][4][LPR], sm_b[TPC][3][4][LPR];        // factors: token, kind (q, k, v), piece of four dims (chunk 0: 0, 1; chunk 1: 2, 3), lane
     __shared__ long long sm_own[TPC];                                    // own row, -1: the token writes no cache row
@@ -285,14 +287,15 @@ extern "C" int trb_paged_append(const trb_paged_t *pool, const trb_batch_t *batc
     p.n_rows = a->n_rows; p.rows_per_seq = a->rows_per_seq; p.hq = a->hq; p.rd = a->rotary_dim; p.interleaved = a->interleaved != 0;
     p.eps = a->eps; p.amplitude = a->amplitude; p.base = make_cursor(&a->base);
     const int heads = (a->q ? a->hq : 0) + 2 * p.c.hkv;
-    // four tokens per CTA and two rounds of heads per warp once that still gives every SM several CTAs
+    // two tokens per CTA and four rounds of heads per warp once that still gives every SM its eight CTAs
     const int rpi = 512 / pool->d;                                        // heads of a warp at a time
-    const bool many = (long long)(a->n_rows / 4) * ((heads + 16 * rpi - 1) / (16 * rpi)) >= 4LL * sm_count();
-    const int tpc = many ? 4 : 1, rows = PA_WARPS * rpi * (many ? 2 : 1);
+    const int wide = 4 * PA_WARPS * rpi;
+    const bool many = (long long)(a->n_rows / 2) * ((heads + wide - 1) / wide) >= 8LL * sm_count();
+    const int tpc = many ? 2 : 1, rows = many ? wide : PA_WARPS * rpi;
     cudaStream_t st = (cudaStream_t)stream;
     pdl_forget(st);
-    TRB_CUDA_CHECK(launch_kernel(pool->d == 256 ? (many ? paged_append_kernel<256, 4, 2> : paged_append_kernel<256, 1, 1>)
-                                                : (many ? paged_append_kernel<128, 4, 2> : paged_append_kernel<128, 1, 1>),
+    TRB_CUDA_CHECK(launch_kernel(pool->d == 256 ? (many ? paged_append_kernel<256, 2, 4> : paged_append_kernel<256, 1, 1>)
+                                                : (many ? paged_append_kernel<128, 2, 4> : paged_append_kernel<128, 1, 1>),
                                  dim3((a->n_rows + tpc - 1) / tpc, (heads + rows - 1) / rows), dim3(PA_THREADS), 0, st, true, p));
     return TRB_OK;
 }
