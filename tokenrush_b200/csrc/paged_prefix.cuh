@@ -79,6 +79,12 @@ paged_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
     const int rows_seq = p.g * p.m, rows_all = p.n_seqs * rows_seq;    // query rows of a kv head
     const int q0 = blk * PX_BM;
     const int rows_here = min(PX_BM, rows_all - q0);
+    // where the block's query rows lie (-1: no row); needs no memory, so it is done before the wait for the launches before this one
+    long long *sm_off = reinterpret_cast<long long *>(sm_mx);          // [128]; read by all before the first tile's maxima are written here
+    if (threadIdx.x < PX_BM) {
+        const int rr = q0 + threadIdx.x, seq = rr / rows_seq, r = rr - seq * rows_seq, i = r / p.g;
+        sm_off[threadIdx.x] = (int)threadIdx.x < rows_here ? (((long long)seq * p.m + i) * p.hq + j * p.g + r - i * p.g) * D : -1;
+    }
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; ++s) {
@@ -255,14 +261,12 @@ paged_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
         // ============ softmax / correction / epilogue: thread = (row, quarter of the keys and of the output columns) ============
         const int row = (warp & 3) * 32 + lane, part = warp >> 2;                  // query row = TMEM lane
         const bool row_ok = row < rows_here, warp_ok = (warp & 3) * 32 < rows_here;
-        const int rr = q0 + (row_ok ? row : 0), seq = rr / rows_seq, r = rr % rows_seq;
-        const long long q_off = (((long long)seq * p.m + r / p.g) * p.hq + j * p.g + r % p.g) * D;
         const uint32_t lane_addr = tmem + ((uint32_t)((warp & 3) * 32) << 16);
         float qinv = 1.f;
         if (n_tiles > 0) {
             if constexpr (!FP8) {
                 // two dims per column, this thread's quarter of the row; rows past the last are zero
-                const uint4 *qp = reinterpret_cast<const uint4 *>(p.q + q_off + part * (D / PX_WG));
+                const uint4 *qp = reinterpret_cast<const uint4 *>(p.q + (row_ok ? sm_off[row] : 0) + part * (D / PX_WG));
                 uint32_t w[D / PX_WG / 2];
 #pragma unroll
                 for (int c = 0; c < D / PX_WG / 8; ++c) {
@@ -275,10 +279,7 @@ paged_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
             } else {
                 // hi + lo e4m3 copies with a power-of-two factor for the row.  A warp takes 8 rows, D / 8 lanes with 16 bytes each per row,
                 // all requested at once: read by the thread that owns the row, the block took most of 20 us
-                long long *sm_off = reinterpret_cast<long long *>(sm_mx);          // [128], then the factors behind it: both are read before tile 0 writes here
-                float *sm_qinv = sm_mx + 2 * PX_BM;
-                if (part == 0) sm_off[row] = row_ok ? q_off : -1;
-                named_barrier(1, PX_SOFTMAX);
+                float *sm_qinv = sm_mx + 2 * PX_BM;                                // behind the offsets
                 constexpr int LPR = D / 8, RPL = 32 / LPR, LOADS = PX_BM / PX_WARPS / RPL;
                 uint4 raw[LOADS];
 #pragma unroll
