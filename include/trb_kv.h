@@ -365,7 +365,7 @@ typedef struct trb_spec_verify_args {
                                     sequences probs_seq_stride apart (elements)                 */
     const void *draft_probs;     /* [n_seqs, k, vocab] likewise, or NULL                        */
     int64_t     probs_seq_stride, probs_row_stride, draft_seq_stride, draft_row_stride;
-    const int64_t *drafts;       /* [n_seqs, k]                                                 */
+    const int64_t *drafts;       /* [n_seqs, k] (may be NULL when k is 0)                       */
     const float *u;              /* [n_seqs, k + 1] numbers in [0, 1)                           */
     const int32_t *n_drafts;     /* [n_seqs] or NULL                                            */
     int64_t    *tokens;          /* [n_seqs, k + 1]: accepted drafts, the new token, then -1    */

@@ -366,10 +366,11 @@ extern "C" int trb_spec_verify(const trb_spec_verify_args_t *a, trb_stream_t str
     p.lens = a->lens; p.lens_width = a->lens_width; p.k = a->k; p.vocab = a->vocab;
     const int64_t strides = a->probs_seq_stride | a->probs_row_stride | (a->draft_probs ? a->draft_seq_stride | a->draft_row_stride : 0);
     p.vec = (((uintptr_t)a->probs | (uintptr_t)a->draft_probs) & 15) == 0 && (strides * size) % 16 == 0;
-    // As many CTAs per row as let all rows run in one wave of three per SM, while a warp's part has a few steps.  (192 rows of
-    // 250000: 2 CTAs each; with 8, 3.5 waves paid the chain draft -> row -> sums -> border one after another.)  16 is the largest cluster.
-    const int steps = (a->vocab + 4096 / size - 1) / (4096 / size);       // (of 512 bytes, for the eight warps of a CTA)
-    int ranks = std::max(1, std::min(std::min(3 * sm_count() / a->n_seqs, 16), steps / 2));
+    // As many CTAs per row as let all rows run in one wave of three per SM, while a warp's part has half a step of 512 bytes.  (192 rows of
+    // 250000: 2 CTAs each; with 8, 3.5 waves paid the chain draft -> row -> sums -> border one after another.)  Clusters of 16, the largest, only
+    // while they leave SMs free: 24 of them do not fit the GPCs at once (24 rows of 16000: 11.0 us, with 8 CTAs 6.9).
+    const int steps = (a->vocab + 4096 / size - 1) / (4096 / size), most = (long long)a->n_seqs * 16 <= sm_count() ? 16 : 8;
+    int ranks = std::max(1, std::min(std::min(3 * sm_count() / a->n_seqs, most), 2 * steps));
     if (ranks > 8 && ranks < 16) ranks = 8;                               // (beyond 8 only 16: the size the device is asked for)
     cudaStream_t st = (cudaStream_t)stream;
     pdl_forget(st);
