@@ -11,7 +11,7 @@
 // 16-byte chunks each, half a row apart: one stream of instructions serves 2 (256 dims) or 4 rows, sums take fewer exchanges, the upper half
 // of a row needs no partner when at most half the head is rotated, and a fully rotated head finds its partners in the same lane.
 // Before its first row a CTA walks a chain of latencies (sequence -> length -> page, angles, factors), so many small ones are resident: two tokens
-// and four warps each, eight CTAs per SM (with four tokens and eight warps, three per SM, 7472 tokens took 59 us, now 51).  Few tokens: one per CTA, one
+// and four warps each, eight CTAs per SM (with four tokens and eight warps, three per SM, 7472 tokens took 59 us, now 50).  Few tokens: one per CTA, one
 // round of heads.
 // The angle is reduced to a fraction of a turn in 64 bits: at position 2e6 an fp32 product is already off by 0.1 rad.
 #include "paged.cuh"
@@ -46,7 +46,7 @@ __device__ __forceinline__ float2 unpack_bf16x2(uint32_t w) { return make_float2
 template <int D, int TPC, int R>
 __global__ void __launch_bounds__(PA_THREADS, 8) paged_append_kernel(const PagedAppendParams p) {
     constexpr int LPR = D / 16, RPI = 32 / LPR;                          // lanes of a row, rows (heads) of a warp
-    __shared__ float4 sm_a[TPC][3][4][LPR], sm_b[TPC][3][4][LPR];        // factors: token, kind (q, k, v), piece of four dims (chunk 0: 0, 1; chunk 1: 2, 3), lane
+    __shared__ float4 sm_a[2 * TPC + 1][4][LPR], sm_b[2 * TPC + 1][4][LPR];    // factors of (token, q or k) and of v; piece of four dims (chunk 0: 0, 1; chunk 1: 2, 3); lane
     __shared__ long long sm_own[TPC];                                    // own row, -1: the token writes no cache row
     __shared__ int sm_page[TPC];
     const int t0 = blockIdx.x * TPC, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, l = lane % LPR;
@@ -108,33 +108,43 @@ __global__ void __launch_bounds__(PA_THREADS, 8) paged_append_kernel(const Paged
         sm_own[threadIdx.x] = own;
         sm_page[threadIdx.x] = page;
     }
-    const int half = p.rd / 2;
+    // ---- the factors, a pair of dims (d, e) per thread and token, its gains loaded once: out_d = x_d g_d c - x_e g_e s, out_e = x_e g_e c + x_d g_d s
+    constexpr int PAIRS = D / 2, GROUPS = PA_THREADS / PAIRS;
+    static_assert(PA_THREADS % PAIRS == 0, "a thread per pair");
+    const int half = p.rd / 2, pair = threadIdx.x % PAIRS;
+    const bool turn = pair < half;
+    const int d = turn && !p.interleaved ? pair : 2 * pair, e = turn && !p.interleaved ? pair + half : d + 1;
+    float gain[2][2];                                                    // q, k; d, e
+#pragma unroll
+    for (int kind = 0; kind < 2; ++kind) {
+        const __nv_bfloat16 *w = kind ? p.kw : p.qw;
+        gain[kind][0] = w ? 1.f + __bfloat162float(w[d]) : 1.f;
+        gain[kind][1] = w ? 1.f + __bfloat162float(w[e]) : 1.f;
+    }
+    const double freq = turn ? p.inv_freq[pair] * 0.15915494309189533577 : 0.0;        // 1 / (2 pi)
+    const long long base = p.rd > 0 ? load_cursor(p.base) : 0;
+    auto put = [&](int at, int dim, float fa, float fb) {                // chunk dim / (D / 2) of lane dim % (D / 2) / 8
+        const int in = dim % (D / 2), piece = dim / (D / 2) * 2 + in % 8 / 4;
+        reinterpret_cast<float *>(&sm_a[at][piece][in / 8])[dim & 3] = fa;
+        reinterpret_cast<float *>(&sm_b[at][piece][in / 8])[dim & 3] = fb;
+    };
+    if (threadIdx.x < PAIRS) {                                           // -0: x * 1 + 0 * -0 is x, a negative zero too
+        put(2 * TPC, d, 1.f, -0.f);
+        put(2 * TPC, e, 1.f, -0.f);
+    }
     __syncthreads();
-    // ---- the factors, a pair of dims (d, e) at a time: out_d = x_d g_d c - x_e g_e s, out_e = x_e g_e c + x_d g_d s
-    for (int x = threadIdx.x; x < TPC * (D / 2); x += PA_THREADS) {
-        const int tk = x / (D / 2), pair = x % (D / 2);
-        float sn = 0.f, cs = 1.f;
-        int d = 2 * pair, e = d + 1;
-        if (pair < half) {
-            const double pos = (double)(load_cursor(p.base) + sm_own[tk]);
-            const double turns = pos * (p.inv_freq[pair] * 0.15915494309189533577);                  // 1 / (2 pi)
+    for (int tk = threadIdx.x / PAIRS; tk < TPC; tk += GROUPS) {
+        float sn = -0.f, cs = 1.f;
+        if (turn) {
+            const double turns = (double)(base + sm_own[tk]) * freq;
             sincospif((float)(2.0 * (turns - rint(turns))), &sn, &cs);
             cs *= p.amplitude;
             sn *= p.amplitude;
-            if (!p.interleaved) { d = pair; e = pair + half; }
         }
-        auto put = [&](int kind, int dim, float fa, float fb) {          // chunk dim / (D / 2) of lane dim % (D / 2) / 8
-            const int in = dim % (D / 2), piece = dim / (D / 2) * 2 + in % 8 / 4;
-            reinterpret_cast<float *>(&sm_a[tk][kind][piece][in / 8])[dim & 3] = fa;
-            reinterpret_cast<float *>(&sm_b[tk][kind][piece][in / 8])[dim & 3] = fb;
-        };
 #pragma unroll
-        for (int kind = 0; kind < 3; ++kind) {
-            const __nv_bfloat16 *w = kind == 0 ? p.qw : kind == 1 ? p.kw : nullptr;
-            const float gd = w ? 1.f + __bfloat162float(w[d]) : 1.f, ge = w ? 1.f + __bfloat162float(w[e]) : 1.f;
-            const bool turn = kind < 2 && pair < half;                   // else -0: x * 1 + 0 * -0 is x, a negative zero too
-            put(kind, d, turn ? gd * cs : gd, turn ? -ge * sn : -0.f);
-            put(kind, e, turn ? ge * cs : ge, turn ? gd * sn : -0.f);
+        for (int kind = 0; kind < 2; ++kind) {
+            put(2 * tk + kind, d, gain[kind][0] * cs, turn ? -gain[kind][1] * sn : -0.f);
+            put(2 * tk + kind, e, gain[kind][1] * cs, turn ? gain[kind][0] * sn : -0.f);
         }
     }
     __syncthreads();
@@ -209,12 +219,13 @@ __global__ void __launch_bounds__(PA_THREADS, 8) paged_append_kernel(const Paged
                 }
             }
             const float2 inv2 = make_float2(inv, inv);
+            const int table = kind == 2 ? 2 * TPC : 2 * tk + kind;
 #pragma unroll
             for (int y = 0; y < 4; ++y) {
-                const float4 fa = sm_a[tk][kind][y][l];
+                const float4 fa = sm_a[table][y][l];
                 float2 u = make_float2(-0.f, -0.f), v = u;
                 if (y < 2 ? lower : upper) {
-                    const float4 fb = sm_b[tk][kind][y][l];
+                    const float4 fb = sm_b[table][y][l];
                     u = __fmul2_rn(unpack_bf16x2(o[2 * y]), make_float2(fb.x, fb.y));
                     v = __fmul2_rn(unpack_bf16x2(o[2 * y + 1]), make_float2(fb.z, fb.w));
                 }
