@@ -48,10 +48,14 @@ template <int D_, bool FP8_> struct PrefixCfg {
     static constexpr int OFF_MX = OFF_FAC + (FP8 ? SLOTS * 3 * BN * 4 : 0);   // [2][PX_WG][128] floats: row maxima of the four quarters
     static constexpr int OFF_BAR = OFF_MX + 2 * PX_WG * PX_BM * 4;
     static constexpr int SMEM = OFF_BAR + 256 + 1024;
-    // weights are staged as 2^(t - reference + LIFT).  The reference of a bf16 pool's row moves only when a score passes it by more than SLACK (a
-    // correction of O waits for the PV before it: 128 readers of 65536 rows 265 -> 245 us); e4m3 weights need the range for precision
-    // (hi + lo keep 8 bits down to 2^-10 of the row's largest weight and 2^-18 of it below; a slack of 3.75 would cost three bits of that and gains 2 %).
-    static constexpr float LIFT = FP8 ? 8.f : 0.f, SLACK = FP8 ? 0.f : 8.f;
+    // Weights are staged as 2^(t - reference + LIFT), and a row's reference follows the largest score of a tile lazily.  bf16 weights keep 8 bits at any
+    // size: the reference moves only when a score passes it by more than SLACK (a correction of O waits for the PV before it: 128 readers of
+    // 65536 rows 265 -> 245 us).  e4m3 weights as hi + lo keep 8 bits down to 2^-10 of the reference and are off by up to 2^-18 of it below, so a
+    // tail far under the largest weight would be lost whatever its mass: the reference also comes down, to within DROP bits of every
+    // tile's own largest score.  What the small weights of a tile lose is then at most 128 * 2^-18 * 2^DROP = 2^-9 of its largest, however many keys there
+    // are (one sink and 65535 keys 18.5 bits below, a piece over all of them: off by 23 % -> 0.4 %; chats 40.4 -> 40.6 us, 128 readers of 65536 rows 230 -> 239, 512 934 -> 1021).
+    // It stops DEPTH bits under the row's largest score, where a tile is worth nothing and O (<= keys * 448 * 2^(LIFT + DEPTH)) still fits fp32.
+    static constexpr float LIFT = FP8 ? 8.f : 0.f, SLACK = 8.f, DROP = 2.f, DEPTH = 40.f;
     static constexpr int TM_S = 0, TM_O = 256, TM_Q = FP8 ? 0 : (D == 256 ? 128 : 384);
     static_assert(SMEM <= 227 * 1024, "shared memory budget");
     static_assert(STAGES * 2 * TILE >= PX_BM * D * 4, "the output block is turned in the ring");
@@ -328,7 +332,7 @@ paged_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
             }
         }
 
-        float m_run = -INFINITY, l_run = 0.f;                                      // l_run: this thread's quarter of the keys
+        float m_run = -INFINITY, m_top = -INFINITY, l_run = 0.f;                   // reference and largest score of the row; l_run: this thread's quarter of the keys
         bool ok = true;
         for (int i = 0; i < n_tiles; ++i) {
             const int b = i & 1;
@@ -372,11 +376,18 @@ paged_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
                 mxbuf[part * PX_BM + row] = fmaxf(fmaxf(mt4[0], mt4[1]), fmaxf(mt4[2], mt4[3]));
                 named_barrier(1, PX_SOFTMAX);
                 const float top = fmaxf(pf_max3(-INFINITY, mxbuf[row], mxbuf[PX_BM + row]), fmaxf(mxbuf[2 * PX_BM + row], mxbuf[3 * PX_BM + row]));
-                const float m_new = top > m_run + C::SLACK ? top : m_run;
-                const float m_safe = m_new == -INFINITY ? 0.f : m_new;
-                const float m_off = m_safe - C::LIFT;
-                const float alpha = m_new == -INFINITY ? 1.f : fast_exp2(m_run - m_safe);
-                // O is corrected only in warps where a row's maximum moved (S of this tile exists, so PV(i - 2) has completed: the
+                float m_new, alpha;
+                if constexpr (!FP8) {
+                    m_new = top > m_run + C::SLACK ? top : m_run;
+                    alpha = m_new == -INFINITY ? 1.f : fast_exp2(m_run - m_new);
+                } else {                                                           // whole references: the factors of their moves are exact
+                    m_top = fmaxf(m_top, top);
+                    m_new = top > m_run || top < m_run - C::DROP ? fmaxf(ceilf(top), ceilf(m_top) - C::DEPTH) : m_run;
+                    const float by = m_run - m_new;                                // <= DEPTH
+                    alpha = m_new == m_run ? 1.f : by > -127.f ? __uint_as_float((uint32_t)((int)by + 127) << 23) : 0.f;
+                }
+                const float m_off = (m_new == -INFINITY ? 0.f : m_new) - C::LIFT;
+                // O is corrected only in warps where a row's reference moved (S of this tile exists, so PV(i - 2) has completed: the
                 // parity cannot be mistaken)
                 if (__any_sync(0xffffffffu, alpha != 1.f) && i > 0) {
                     ok = __all_sync(0xffffffffu, mbar_wait(o_done, (i - 1) & 1));
