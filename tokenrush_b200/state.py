@@ -63,7 +63,8 @@ class State:
 class PagedState:
     """Preallocated paged KV state of a batch: one pool of pages for every layer, `[layer, page, kv_head, row, head_dim]` in bf16 or
     e4m3 with fp32 scales, a page table and lengths on the device, and the pages of a prefix that all sequences share.
-    Pages are handed out on the host; lengths live on the device (`fused.spec_verify` advances them there), so a
+    Pages are handed out on the host, and table entries that name none are -1 (a step that goes past a sequence's pages is reported as
+    ST_CURSOR_RANGE and writes nothing there); lengths live on the device (`fused.spec_verify` advances them there), so a
     captured step keeps working while sequences come, grow and leave.  Counterpart of `State` for `fused.paged_append`
     and `fused.attn_paged`."""
 
@@ -80,9 +81,9 @@ class PagedState:
         self.v = torch.zeros_like(self.k)
         self.k_scale = torch.ones(self.k.shape[:4], device=device, dtype=torch.float32) if self.fp8 else None
         self.v_scale = torch.ones_like(self.k_scale) if self.fp8 else None
-        self.table = torch.zeros(max_seqs, max_pages, device=device, dtype=torch.int32)
+        self.table = torch.full((max_seqs, max_pages), -1, device=device, dtype=torch.int32)
         self.lens = torch.full((max_seqs,), -1, device=device, dtype=torch.long)      # -1: an empty slot
-        self.prefix_table = torch.zeros(max_prefix_pages, device=device, dtype=torch.int32) if max_prefix_pages else None
+        self.prefix_table = torch.full((max_prefix_pages,), -1, device=device, dtype=torch.int32) if max_prefix_pages else None
         self.prefix_len = torch.zeros(1, device=device, dtype=torch.long)
         self.attn_slot = {l: i for i, l in enumerate(layers)}
         self._free = list(range(num_pages - 1, -1, -1))
@@ -133,6 +134,7 @@ class PagedState:
             raise ValueError(f"slot {seq} is empty")
         self._free += reversed(self._own[seq])
         self._own[seq] = None
+        self.table[seq] = -1
         self.lens[seq] = -1
 
     def set_prefix(self, rows: int):
@@ -146,5 +148,6 @@ class PagedState:
         if want < len(self._prefix):
             self._free += reversed(self._prefix[want:])
             del self._prefix[want:]
+            self.prefix_table[want:] = -1
         self._grow(self._prefix, self.prefix_table, rows)
         self.prefix_len.fill_(rows)
