@@ -162,9 +162,11 @@ Tensor attn_paged(const Tensor &q, const Tensor &k_pages, const Tensor &v_pages,
         need(!a.prefix_len.dev && a.prefix_len.host == 0, "a prefix needs its prefix_table");
     }
     if (gate) {
-        need(gate->sizes() == q.sizes() && gate->scalar_type() == at::kBFloat16 && gate->stride(3) == 1 && gate->stride(0) == a.m * gate->stride(1),
+        need(gate->sizes() == q.sizes() && gate->scalar_type() == at::kBFloat16 && gate->stride(3) == 1 &&
+                 (batch.n_seqs == 1 || a.m == 1 || gate->stride(0) == a.m * gate->stride(1)),
              "gate must be a bf16 [B, M, HQ, D] view with equally spaced rows");
-        a.gate = ptr(gate); a.gate_row_stride = gate->stride(1); a.gate_head_stride = gate->stride(2);
+        // (the stride of a dim of size 1 means nothing)
+        a.gate = ptr(gate); a.gate_row_stride = gate->stride(a.m == 1 ? 0 : 1); a.gate_head_stride = gate->stride(2);
     }
     Tensor out;
     if (out_given) {
