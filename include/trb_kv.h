@@ -344,10 +344,12 @@ typedef struct trb_attn_paged_args {
     void       *workspace;       /* trb_attn_paged_workspace_bytes() bytes, any contents        */
     size_t      workspace_bytes;
 } trb_attn_paged_args_t;
-/* The prefix is read by a kernel of its own when the scans of all sequences together would read at least min_bytes of it; a negative
+/* The prefix is read by a kernel of its own when the scans of all sequences together would read at least min_bytes of it, going by prefix_len
+ * where it is a host value and by the whole prefix_table where it is on the device (pass the table's pages in use then); a negative
  * value restores the default (72 MB).  Both ways give results within the same tolerance; the switch exists for testing and
  * measurement, and a workspace has to be sized under the setting it is used with. */
 int trb_set_paged_prefix_bytes(int64_t min_bytes);
+/* enough for every prefix_len up to prefix_pages pages */
 size_t trb_attn_paged_workspace_bytes(const trb_paged_t *pool, int32_t n_seqs, int32_t m, int32_t hq, int32_t prefix_pages);
 int trb_attn_paged(const trb_paged_t *pool, const trb_batch_t *batch, const trb_attn_paged_args_t *args, trb_stream_t stream);
 

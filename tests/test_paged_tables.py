@@ -72,3 +72,11 @@ def test_a_step_past_the_reservation_is_reported_and_writes_nothing():
     q = torch.randn(3, 2, 4, 128, device="cuda", generator=g).bfloat16()
     tb.fused.attn_paged(q, k, v, st.table, st.lens)
     assert tb._lib.device_status() == tb._lib.ST_CURSOR_RANGE
+
+
+def test_prefix_pages_are_those_in_use():
+    st = state("cpu")
+    assert st.prefix_pages.tolist() == []
+    for rows, n in ((40, 3), (17, 2), (0, 0), (1, 1)):
+        st.set_prefix(rows)
+        assert st.prefix_pages.tolist() == st.prefix_table[:n].tolist() and len(st.prefix_pages) == n and -1 not in st.prefix_pages.tolist()

@@ -157,6 +157,7 @@ Tensor attn_paged(const Tensor &q, const Tensor &k_pages, const Tensor &v_pages,
         a.prefix_pages = (int32_t)prefix_table->size(0);
         if (!a.prefix_len.dev)
             need(a.prefix_len.host >= 0 && a.prefix_len.host <= (int64_t)a.prefix_pages * pool.page_size, "prefix_len exceeds the pages of prefix_table");
+        if (!a.prefix_len.dev && pool.page_size > 0) a.prefix_pages = (int32_t)((a.prefix_len.host + pool.page_size - 1) / pool.page_size);      // the pages in use
         if (a.prefix_pages) a.prefix_table = (const int32_t *)ptr(prefix_table);
     } else {
         need(!a.prefix_len.dev && a.prefix_len.host == 0, "a prefix needs its prefix_table");

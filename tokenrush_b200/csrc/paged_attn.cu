@@ -646,7 +646,8 @@ __global__ void __launch_bounds__(256) paged_merge_kernel(const PagedAttnParams 
     else *reinterpret_cast<uint2 *>(dst) = *reinterpret_cast<const uint2 *>(ob);
 }
 
-// Bytes that the scans of all sequences would read of the prefix from which on it is read once, by a kernel of its own.  That kernel costs 8
+// Bytes that the scans of all sequences would read of the prefix from which on it is read once, by a kernel of its own.  Its rows are those of
+// prefix_len where the host knows it; a length on the device counts as a full table (the launches are chosen before it can be read).  That kernel costs 8
 // to 12 us before it pays.  Measured with / without it (us; own rows 100 - 300): 24/4 heads x 256 e4m3, 8 sequences over 4096 rows (68 MB)
 // 23.4 / 20.6, 16 over 4096 (136 MB) 25.5 / 29.3, 32 over 16384 43 / 137; bf16 4 over 4096 (67 MB) 17.6 / 17.1, 8 over 4096 (134 MB) 19.5 / 25.2;
 // 32/8 x 128 e4m3, 8 over 4096 (69 MB) 19.8 / 20.7; 16/16 x 128 bf16, 8 over 1024 (67 MB) 16.0 / 16.1; 32 over 256 (33 MB) 24.7 / 17.8.
@@ -760,7 +761,9 @@ extern "C" int trb_attn_paged(const trb_paged_t *pool, const trb_batch_t *batch,
     if (((((long long)a->prefix_pages + batch->table_pages) << p.c.page_shift) / 16 + 2 + PS_TURN) * batch->n_seqs > 0x7fffffffLL) return TRB_E_UNSUPPORTED;
     if ((((uintptr_t)a->q | (uintptr_t)a->out) & 15) || ((uintptr_t)a->workspace & 255) || ((uintptr_t)a->prefix_table & 3) || ((uintptr_t)a->gate & 1)) return TRB_E_ALIGN;
     const bool fp8 = p.c.ks != nullptr;
-    const PagedAttnPlan plan = paged_attn_plan(pool->d, fp8, pool->hkv, a->hq, batch->n_seqs, a->m, (long long)a->prefix_pages << p.c.page_shift);
+    long long prefix_rows = (long long)a->prefix_pages << p.c.page_shift;
+    if (a->prefix_pages > 0 && !a->prefix_len.dev) prefix_rows = std::max(0LL, std::min(prefix_rows, (long long)a->prefix_len.host));
+    const PagedAttnPlan plan = paged_attn_plan(pool->d, fp8, pool->hkv, a->hq, batch->n_seqs, a->m, prefix_rows);
     if (a->workspace_bytes < plan.bytes) return TRB_E_CAPACITY;
     p.q = (const __nv_bfloat16 *)a->q; p.out = (__nv_bfloat16 *)a->out; p.gate = (const __nv_bfloat16 *)a->gate;
     p.gate_rs = a->gate_row_stride; p.gate_hs = a->gate_head_stride;

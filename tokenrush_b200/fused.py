@@ -353,7 +353,8 @@ def paged_append(k, v, k_pages, v_pages, table, lens, k_scale=None, v_scale=None
 def attn_paged(q, k_pages, v_pages, table, lens, k_scale=None, v_scale=None, *, prefix_table=None, prefix_len=0, gate=None, scale=None, out=None):
     """Attention of a step's new rows over a paged cache: q [B, M, HQ, D] bf16 (from paged_append; the M rows are already
     appended, lens is still the length before them).  Row i of sequence b sees the prefix_len rows that all sequences
-    share (pages prefix_table [P] int32; prefix_len: an int or a device integer) and its own rows <= lens[b] + i.  Slots with
+    share (pages prefix_table [P] int32; prefix_len: an int, or a device integer, whose
+    call is planned for all pages of prefix_table: give it those in use, PagedState.prefix_pages) and its own rows <= lens[b] + i.  Slots with
     lens[b] < 0 give zeros.  gate (optional): bf16 [B, M, HQ, D] view, out = bf16(o) * bf16(sigmoid(gate)) as in attn_decode_fused.
     Returns [B, M, HQ, D].  Lengths are read on the device, so a captured step serves all of them."""
     return (L._native or L.native()).attn_paged(q, k_pages, v_pages, table, lens, k_scale, v_scale, prefix_table, prefix_len, gate, scale, out)

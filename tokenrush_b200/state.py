@@ -100,6 +100,12 @@ class PagedState:
     def free_pages(self) -> int:
         return len(self._free)
 
+    @property
+    def prefix_pages(self):
+        """The entries of prefix_table in use, the form for `fused.attn_paged`, which reads a long prefix otherwise than a short one.  A captured
+        step keeps the number of entries that it was captured with."""
+        return self.prefix_table[:len(self._prefix)] if self.prefix_table is not None else None
+
     def _grow(self, pages: list, table: torch.Tensor, rows: int):
         want = -(-rows // self.page_size)
         if want > table.shape[0]:
