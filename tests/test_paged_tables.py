@@ -80,3 +80,24 @@ def test_prefix_pages_are_those_in_use():
     for rows, n in ((40, 3), (17, 2), (0, 0), (1, 1)):
         st.set_prefix(rows)
         assert st.prefix_pages.tolist() == st.prefix_table[:n].tolist() and len(st.prefix_pages) == n and -1 not in st.prefix_pages.tolist()
+
+
+@pytest.mark.gpu
+def test_a_state_without_room_for_a_prefix_serves_the_same_calls():
+    import tokenrush_b200 as tb
+    st = PagedState(Cfg, num_pages=4, max_seqs=2, max_pages=2, page_size=16, device="cuda")
+    k, v, _, _ = st.layer(0)
+    st.open(0, 5)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    rows = torch.randn(10, 2, 128, device="cuda", generator=g).bfloat16()
+    tb.fused.paged_append(rows, rows, k, v, st.table, st.lens, base=st.prefix_len)
+    q = torch.randn(2, 5, 4, 128, device="cuda", generator=g).bfloat16()
+    got = tb.fused.attn_paged(q, k, v, st.table, st.lens, prefix_table=st.prefix_table, prefix_len=st.prefix_len)
+    assert torch.equal(got, tb.fused.attn_paged(q, k, v, st.table, st.lens)) and tb._lib.device_status() == 0
+
+
+def test_a_state_without_room_for_a_prefix_refuses_one():
+    st = PagedState(Cfg, num_pages=4, max_seqs=2, max_pages=2, page_size=16, device="cpu")
+    for rows in (0, 1):
+        with pytest.raises(ValueError):
+            st.set_prefix(rows)

@@ -83,7 +83,7 @@ class PagedState:
         self.v_scale = torch.ones_like(self.k_scale) if self.fp8 else None
         self.table = torch.full((max_seqs, max_pages), -1, device=device, dtype=torch.int32)
         self.lens = torch.full((max_seqs,), -1, device=device, dtype=torch.long)      # -1: an empty slot
-        self.prefix_table = torch.full((max_prefix_pages,), -1, device=device, dtype=torch.int32) if max_prefix_pages else None
+        self.prefix_table = torch.full((max_prefix_pages,), -1, device=device, dtype=torch.int32)     # (no entries: no room for a prefix)
         self.prefix_len = torch.zeros(1, device=device, dtype=torch.long)
         self.attn_slot = {l: i for i, l in enumerate(layers)}
         self._free = list(range(num_pages - 1, -1, -1))
@@ -104,7 +104,7 @@ class PagedState:
     def prefix_pages(self):
         """The entries of prefix_table in use, the form for `fused.attn_paged`, which reads a long prefix otherwise than a short one.  A captured
         step keeps the number of entries that it was captured with."""
-        return self.prefix_table[:len(self._prefix)] if self.prefix_table is not None else None
+        return self.prefix_table[:len(self._prefix)]
 
     def _grow(self, pages: list, table: torch.Tensor, rows: int):
         want = -(-rows // self.page_size)
@@ -148,7 +148,7 @@ class PagedState:
         sequence is open: their positions count from its end."""
         if any(p is not None for p in self._own):
             raise ValueError("the prefix can only change while every slot is empty")
-        if self.prefix_table is None:
+        if not len(self.prefix_table):
             raise ValueError("made without room for a prefix (max_prefix_pages)")
         want = -(-rows // self.page_size)
         if want < len(self._prefix):
