@@ -101,3 +101,13 @@ def test_a_state_without_room_for_a_prefix_refuses_one():
     for rows in (0, 1):
         with pytest.raises(ValueError):
             st.set_prefix(rows)
+
+
+def test_a_negative_prefix_is_refused():
+    st = state("cpu")
+    st.set_prefix(40)
+    for rows in (-1, -40):
+        with pytest.raises(ValueError):
+            st.set_prefix(rows)
+        holds(st)
+        assert int(st.prefix_len) == 40 and len(st._prefix) == 3

@@ -150,6 +150,8 @@ class PagedState:
             raise ValueError("the prefix can only change while every slot is empty")
         if not len(self.prefix_table):
             raise ValueError("made without room for a prefix (max_prefix_pages)")
+        if rows < 0:
+            raise ValueError("a prefix has no negative number of rows")
         want = -(-rows // self.page_size)
         if want < len(self._prefix):
             self._free += reversed(self._prefix[want:])
