@@ -120,6 +120,27 @@ __device__ __forceinline__ bool mbar_wait(uint64_t *bar, uint32_t parity) {
     return false;
 }
 
+// Waits for a copy or product already under way, before the memory that it uses is given up.  It ends by itself, so the limit
+// (some seconds) is a last bound that no setting shortens.
+__device__ __forceinline__ void mbar_drain(uint64_t *bar, uint32_t parity) {
+    for (uint32_t it = 0; it < (1u << 20); ++it) {
+        if (mbar_try_wait(bar, parity)) return;
+        if (it > 64) __nanosleep(64);
+    }
+    raise_status(TRB_ST_WAIT_TIMEOUT);
+}
+// mbar_wait of a whole warp, with one answer for all its lanes: a lane whose wait ran out beside others that go on would leave them at their
+// next warp barrier.
+__device__ __forceinline__ bool mbar_wait_warp(uint64_t *bar, uint32_t parity) {
+    const uint32_t limit = c_wait_limit[0];
+    for (uint32_t it = 0; it < limit; ++it) {
+        if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+        if (it > 64) __nanosleep(64);
+    }
+    raise_status(TRB_ST_WAIT_TIMEOUT);
+    return false;
+}
+
 // ------------------------------------------------------------------------------ TMA
 __device__ __forceinline__ void tma_prefetch_desc(const CUtensorMap *m) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(m)) : "memory");

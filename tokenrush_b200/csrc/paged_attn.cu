@@ -101,7 +101,7 @@ paged_scan_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
     const int rows = p.g * p.m, r0 = grp * 8 * NS;
     const uint32_t ring = smem_u32(ps_smem + warp * C::RING), scales = smem_u32(ps_smem + C::OFF_SC) + warp * STAGES * SUB * 128;
     uint64_t *full = reinterpret_cast<uint64_t *>(ps_smem + C::OFF_BAR) + warp * 4;      // one per stage
-    uint32_t phases = 0;                                               // bit s: parity of stage s's next completion
+    uint32_t phases = 0, armed = 0;                                    // bit s: parity of stage s's next completion; of the one after its last load
     bool ok = true;                                                    // no wait of this warp has run out
     if (lane == 0) {
         for (int s = 0; s < STAGES; ++s) mbar_init(&full[s], 1u);
@@ -213,7 +213,10 @@ paged_scan_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
 #pragma unroll
         for (int sb = 0; sb < SUB; ++sb) now[sb] = pages[sb];
         fetch_pages(k + 1);
-        if (k < steps && ok) load_step(s0 + warp + k * PS_WARPS, (k + RED) % STAGES, now);
+        if (k < steps && ok) {
+            load_step(s0 + warp + k * PS_WARPS, (k + RED) % STAGES, now);
+            armed ^= 1u << (k + RED) % STAGES;
+        }
     };
     // ---- the query rows as MMA fragments: step (jj, w) of lane (g, t) holds dims of chunk 8 (jj / 2) + 2 t + jj % 2 (so that the eight lanes
     // of a shared-memory phase, two rows by four t, meet eight different places of the swizzle).  e4m3: f16 with a power-of-two
@@ -312,9 +315,9 @@ paged_scan_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
         for (int k = 0; k < steps; ++k) {
             request(k + STAGES - 1);
             const int stage = (k + RED) % STAGES, step = s0 + warp + k * PS_WARPS;
-            ok = __all_sync(0xffffffffu, mbar_wait(&full[stage], (phases >> stage) & 1u));
+            ok = mbar_wait_warp(&full[stage], (phases >> stage) & 1u);
             if (!ok) steps = 0;                                        // (the output is undefined, but nothing hangs)
-            phases ^= 1u << stage;
+            phases ^= (uint32_t)ok << stage;
             const uint32_t base = ring + stage * C::STAGE;
 #pragma unroll
             for (int sb = 0; sb < SUB; ++sb) {                         // V rows behind the last one: a weight of zero times NaN must not reach O
@@ -490,6 +493,11 @@ paged_scan_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
                 }
             }
             __syncwarp();                                              // the stage may be refilled
+        }
+        if (!ok) {                                                     // no copy may land in the exchange below, or after the CTA has left
+            for (int s = 0; s < STAGES; ++s)
+                if ((armed ^ phases) >> s & 1u) mbar_drain(&full[s], (phases >> s) & 1u);
+            armed = phases;
         }
         // every step of this sequence has been consumed: on to the next one that has some in this CTA's piece
         do ++seq; while (seq < p.b.n_seqs && sm_cnt[seq + 1] <= sm_cnt[seq]);

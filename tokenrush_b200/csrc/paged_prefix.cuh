@@ -74,9 +74,9 @@ paged_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
     uint64_t *bars = reinterpret_cast<uint64_t *>(smem + C::OFF_BAR);
     // K and V tiles have barriers of their own: a K tile is refilled as soon as its product has run
     uint64_t *k_full = bars, *v_full = k_full + STAGES, *k_free = v_full + STAGES, *v_free = k_free + STAGES;
-    uint64_t *s_full = v_free + STAGES, *p_full = s_full + 2, *o_done = p_full + 2, *o_last = o_done + 1, *q_ready = o_last + 1, *fac_full = q_ready + 1;
+    uint64_t *s_full = v_free + STAGES, *p_full = s_full + 2, *o_done = p_full + 2, *o_last = o_done + 1, *q_ready = o_last + 1, *mma_out = q_ready + 1, *v_clean = mma_out + 1, *fac_full = v_clean + 1;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(fac_full + SLOTS);
-    static_assert((4 * C::STAGES + 7 + C::SLOTS) * 8 + 4 <= 256, "barriers");
+    static_assert((4 * C::STAGES + 9 + C::SLOTS) * 8 + 4 <= 256, "barriers");
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int split = blockIdx.x % p.splits, blk = blockIdx.x / p.splits % p.blocks, j = blockIdx.x / p.splits / p.blocks;
@@ -99,7 +99,7 @@ paged_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
         // phase of one barrier would hide the first from its parity
         for (int b = 0; b < 2; ++b) { mbar_init(&s_full[b], 1u); mbar_init(&p_full[b], PX_WARPS); }
         for (int b = 0; b < SLOTS; ++b) mbar_init(&fac_full[b], 1u);
-        mbar_init(o_done, 1u); mbar_init(o_last, 1u); mbar_init(q_ready, PX_WARPS);
+        mbar_init(o_done, 1u); mbar_init(o_last, 1u); mbar_init(q_ready, PX_WARPS); mbar_init(mma_out, 1u); mbar_init(v_clean, 1u);
         mbar_fence_init();
         tma_prefetch_desc(&tm_k); tma_prefetch_desc(&tm_v);
     }
@@ -127,7 +127,7 @@ paged_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
             return p.table[row >> p.c.page_shift];
         };
         auto build_factors = [&](int t) -> bool {
-            if (!mbar_wait(&k_full[t % STAGES], (t / STAGES) & 1)) return false;   // the tile's scales have landed
+            if (!mbar_wait_warp(&k_full[t % STAGES], (t / STAGES) & 1)) return false;      // the tile's scales have landed
             float *fn = sm_fac + (t % SLOTS) * 3 * BN;
             const float *sc = sm_sc + (t % SLOTS) * 2 * BN;
 #pragma unroll
@@ -152,8 +152,10 @@ paged_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
             const int boxes = min(per_tile, (n_prefix - row0 + box - 1) / box);     // boxes with live rows: the others are not loaded
             uint8_t *kt = smem + C::OFF_KV + s * 2 * TILE, *vt = kt + TILE;
             const uint32_t par = ((i / STAGES) & 1) ^ 1;
-            // box b, column block sg of this tile: its page is that of the box's first 16 keys; a page outside the pool reads zeros
-            auto load = [&](uint8_t *dst, const CUtensorMap *map, uint64_t *bar) {
+            // box b, column block sg of this tile: its page is that of the box's first 16 keys; a page outside the pool reads zeros.
+            // The stage is free once the product with its last tile has run
+            auto load = [&](uint8_t *dst, const CUtensorMap *map, uint64_t *bar, uint64_t *free) -> bool {
+                if (i >= STAGES && !mbar_wait_warp(free, par)) return false;
                 if (lane == 0) mbar_arrive_expect_tx(bar, boxes * box * C::ROWB);
                 __syncwarp();
                 for (int x0 = 0; x0 < per_tile * SEGS; x0 += 32) {
@@ -163,9 +165,9 @@ paged_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
                         tma_load_4d(dst + sg * (BN * 128) + b * box * 128, map, bar, 0, sg, (row0 + b * box) & page_mask, pg < 0 ? -1 : pg * p.c.hkv + j);
                 }
                 __syncwarp();
+                return true;
             };
-            if (i >= STAGES && !mbar_wait(&k_free[s], par)) break;                 // the product with the stage's last K tile has run
-            load(kt, &tm_k, &k_full[s]);
+            if (!load(kt, &tm_k, &k_full[s], &k_free[s])) break;
             ++k_sent;
             if constexpr (FP8) {
                 float *sc = sm_sc + (i % SLOTS) * 2 * BN;
@@ -180,28 +182,40 @@ paged_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
                 cp_async_mbar_arrive_noinc(&k_full[s]);
                 if (i >= 1 && !build_factors(i - 1)) break;
             }
-            if (i >= STAGES && !mbar_wait(&v_free[s], par)) break;
-            load(vt, &tm_v, &v_full[s]);
+            if (!load(vt, &tm_v, &v_full[s], &v_free[s])) break;
             ++v_sent;
         }
         if constexpr (FP8) { if (n_tiles > 0) build_factors(n_tiles - 1); }
+        if (n_tiles > 0 && v_sent == n_tiles && left_last < BN) {                  // V rows behind the prefix: 0 * NaN must not reach O
+            const int s = (n_tiles - 1) % STAGES;
+            uint8_t *v_tile = smem + C::OFF_KV + s * 2 * TILE + TILE;
+            if (mbar_wait_warp(&v_full[s], ((n_tiles - 1) / STAGES) & 1)) {
+                for (int x = lane; x < (BN - left_last) * SEGS * 8; x += 32) {
+                    const int row = left_last + x / (SEGS * 8), sg = x / 8 % SEGS;
+                    *reinterpret_cast<uint4 *>(v_tile + sg * (BN * 128) + row * 128 + (x & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+                }
+                fence_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(v_clean);
+            }
+        }
         // no copy is on its way when the CTA leaves, also after a wait that ran out
-        for (int t = max(0, k_sent - STAGES); t < k_sent; ++t) mbar_wait(&k_full[t % STAGES], (t / STAGES) & 1);
-        for (int t = max(0, v_sent - STAGES); t < v_sent; ++t) mbar_wait(&v_full[t % STAGES], (t / STAGES) & 1);
+        for (int t = max(0, k_sent - STAGES); t < k_sent; ++t) mbar_drain(&k_full[t % STAGES], (t / STAGES) & 1);
+        for (int t = max(0, v_sent - STAGES); t < v_sent; ++t) mbar_drain(&v_full[t % STAGES], (t / STAGES) & 1);
     } else if (warp == PX_WARPS + 1) {
-        // ================================ MMA issuer ==================================
+        // ================================ MMA issuer: one thread ==================================
         // QK(0), QK(1), PV(0), QK(2), PV(1), ..: the pipe runs in order of issue, so QK(i + 2) overwrites the buffer that holds
         // P(i) only after PV(i) has read it
-        const uint32_t q_tm = tmem + C::TM_Q;
-        const uint32_t q_hi = smem_u32(smem), q_lo = q_hi + C::Q_BYTES;
-        constexpr uint32_t IDESC_QK = FP8 ? umma_idesc_f8(PX_BM, BN, false, false) : umma_idesc_bf16(PX_BM, BN, false, false);
-        constexpr uint32_t IDESC_PV = FP8 ? umma_idesc_f8(PX_BM, D, false, true) : umma_idesc_bf16(PX_BM, D, false, true);
-        auto issue_qk = [&](int i) -> bool {
-            const int s = i % STAGES, b = i & 1;
-            const uint32_t kt = smem_u32(smem + C::OFF_KV + s * 2 * TILE);
-            if (!mbar_wait(&k_full[s], (i / STAGES) & 1)) return false;
-            tc_fence_after();
-            if (lane == 0) {
+        if (lane == 0 && n_tiles > 0) {
+            const uint32_t q_tm = tmem + C::TM_Q;
+            const uint32_t q_hi = smem_u32(smem), q_lo = q_hi + C::Q_BYTES;
+            constexpr uint32_t IDESC_QK = FP8 ? umma_idesc_f8(PX_BM, BN, false, false) : umma_idesc_bf16(PX_BM, BN, false, false);
+            constexpr uint32_t IDESC_PV = FP8 ? umma_idesc_f8(PX_BM, D, false, true) : umma_idesc_bf16(PX_BM, D, false, true);
+            auto issue_qk = [&](int i) -> bool {
+                const int s = i % STAGES, b = i & 1;
+                const uint32_t kt = smem_u32(smem + C::OFF_KV + s * 2 * TILE);
+                if (!mbar_wait(&k_full[s], (i / STAGES) & 1)) return false;
+                tc_fence_after();
                 if constexpr (FP8) {
 #pragma unroll
                     for (int term = 0; term < 2; ++term)
@@ -221,29 +235,17 @@ paged_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
                 }
                 tc_commit(&k_free[s]);
                 tc_commit(&s_full[b]);
-            }
-            __syncwarp();
-            return true;
-        };
-        bool ok = n_tiles > 0 && mbar_wait(q_ready, 0);
-        if (ok) ok = issue_qk(0);
-        for (int i = 0; i < n_tiles && ok; ++i) {
-            const int s = i % STAGES;
-            uint8_t *v_tile = smem + C::OFF_KV + s * 2 * TILE + TILE;
-            const uint32_t vt = smem_u32(v_tile), p_tm = tmem + C::TM_S + (i & 1) * BN;
-            if (i + 1 < n_tiles && !(ok = issue_qk(i + 1))) break;
-            if (!(ok = mbar_wait(&v_full[s], (i / STAGES) & 1))) break;
-            if (i == n_tiles - 1 && left_last < BN) {                              // rows behind the prefix: 0 * NaN must not reach O
-                for (int x = lane; x < (BN - left_last) * SEGS * 8; x += 32) {
-                    const int row = left_last + x / (SEGS * 8), sg = x / 8 % SEGS;
-                    *reinterpret_cast<uint4 *>(v_tile + sg * (BN * 128) + row * 128 + (x & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
-                }
-                fence_async_smem();
-                __syncwarp();
-            }
-            if (!(ok = mbar_wait(&p_full[i & 1], (i >> 1) & 1))) break;                           // P staged, O corrected
-            tc_fence_after();
-            if (lane == 0) {
+                return true;
+            };
+            bool ok = mbar_wait(q_ready, 0) && issue_qk(0);
+            for (int i = 0; i < n_tiles && ok; ++i) {
+                const int s = i % STAGES;
+                const uint32_t vt = smem_u32(smem + C::OFF_KV + s * 2 * TILE + TILE), p_tm = tmem + C::TM_S + (i & 1) * BN;
+                if (i + 1 < n_tiles && !(ok = issue_qk(i + 1))) break;
+                if (!(ok = mbar_wait(&v_full[s], (i / STAGES) & 1))) break;
+                if (i == n_tiles - 1 && left_last < BN && !(ok = mbar_wait(v_clean, 0))) break;
+                if (!(ok = mbar_wait(&p_full[i & 1], (i >> 1) & 1))) break;        // P staged, O corrected
+                tc_fence_after();
                 if constexpr (FP8) {
 #pragma unroll
                     for (int term = 0; term < 2; ++term)
@@ -259,7 +261,9 @@ paged_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
                 tc_commit(&v_free[s]);
                 tc_commit(i == n_tiles - 1 ? o_last : o_done);
             }
-            __syncwarp();
+            // no product is under way when the tensor memory is given back, also after a wait that ran out
+            tc_commit(mma_out);
+            mbar_drain(mma_out, 0);
         }
     } else {
         // ============ softmax / correction / epilogue: thread = (row, quarter of the keys and of the output columns) ============
@@ -390,7 +394,7 @@ paged_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
                 // O is corrected only in warps where a row's reference moved (S of this tile exists, so PV(i - 2) has completed: the
                 // parity cannot be mistaken)
                 if (__any_sync(0xffffffffu, alpha != 1.f) && i > 0) {
-                    ok = __all_sync(0xffffffffu, mbar_wait(o_done, (i - 1) & 1));
+                    ok = mbar_wait_warp(o_done, (i - 1) & 1);
                     if (ok) {
                         tc_fence_after();
 #pragma unroll 1
