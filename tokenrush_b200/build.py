@@ -41,10 +41,15 @@ LIB_TIMELINE = os.path.join(HERE, "libtrb_kv_timeline.so")
 BINDING = os.path.join(HERE, "_binding.so")
 
 
+def binding_sources():
+    import torch
+    # (the binding is built against one torch: another one, installed later, makes it out of date)
+    return [os.path.join(CSRC, "binding.cpp"), os.path.join(HERE, "..", "include", "trb_kv.h"), os.path.join(os.path.dirname(torch.__file__), "version.py")]
+
+
 def build_binding(force: bool = False) -> str:
     src = os.path.join(CSRC, "binding.cpp")
-    deps = [src, os.path.join(HERE, "..", "include", "trb_kv.h")]
-    if not force and os.path.exists(BINDING) and all(os.path.getmtime(d) <= os.path.getmtime(BINDING) for d in deps):
+    if not force and os.path.exists(BINDING) and all(os.path.getmtime(d) <= os.path.getmtime(BINDING) for d in binding_sources()):
         return BINDING
     import sysconfig
     import torch
