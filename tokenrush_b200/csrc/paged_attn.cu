@@ -450,11 +450,11 @@ paged_scan_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constan
                     for (int h = 0; h < 2; ++h) {
                         uint32_t pk;
                         if constexpr (FP8) {
-                            pk = pack_f16x2(w[2 * h], w[2 * h + 1]);
+                            pk = pack_f16x2(w[2 * h], w[2 * h + 1]);      // 11 bits down to 2^-14 of the reference, off by 2^-25 of it below
 #pragma unroll
                             for (int e = 0; e < 2; ++e) l[s * 2 + e] += w[2 * h + e] > 0.f ? w[2 * h + e] * vinv[sb][h] : w[2 * h + e] * 0.f;
                         } else {
-                            // the sum takes the weights as they multiply V
+                            // bf16 like the V they multiply (one MMA takes one type, f16 cannot hold V): 8 bits at any size.  The sum takes them as they are then
                             pk = pack_bf16x2(w[2 * h], w[2 * h + 1]);
                             const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&pk));
                             l[s * 2] += f.x;

@@ -8,12 +8,15 @@ argument meaning, backed by the sm_100a CUDA library through its C ABI.
     attn_window_block    tokenrush/fused.py:600-622
     add_rmsnorm          tokenrush/fused.py:48-60    (the step after the attention output projection)
 
-For batches of sequences (the reference serves one) over a paged cache: `paged_append`, `attn_paged` and
-`spec_verify`, the batch's prep, decode and commit,
-plus the cursor arithmetic the reference does with small torch ops (`spec_commit`,
+with the cursor arithmetic the reference does with small torch ops (`spec_commit`,
 tokenrush/model.py:306-312) and the ring write of the DFlash draft cache (`ring_write`,
-tokenrush/dflash.py:293-294).  Every call launches on torch's current stream, allocates
-only its outputs (with torch, so it is legal under graph capture) and never synchronises.
+tokenrush/dflash.py:293-294).
+
+For batches of sequences (the reference serves one) over a paged cache: `paged_append`, `attn_paged` and
+`spec_verify`, the batch's prep, decode and commit.
+
+Every call launches on torch's current stream, allocates its outputs and `attn_paged` its workspace with torch
+(legal under graph capture; the decode's workspaces are made once, outside capture) and never synchronises.
 There is no fallback: a CUDA tensor and the built library are required.
 """
 from __future__ import annotations
@@ -353,9 +356,9 @@ def paged_append(k, v, k_pages, v_pages, table, lens, k_scale=None, v_scale=None
 def attn_paged(q, k_pages, v_pages, table, lens, k_scale=None, v_scale=None, *, prefix_table=None, prefix_len=0, gate=None, scale=None, out=None):
     """Attention of a step's new rows over a paged cache: q [B, M, HQ, D] bf16 (from paged_append; the M rows are already
     appended, lens is still the length before them).  Row i of sequence b sees the prefix_len rows that all sequences
-    share (pages prefix_table [P] int32; prefix_len: an int, or a device integer, whose
-    call is planned for all pages of prefix_table: give it those in use, PagedState.prefix_pages) and its own rows <= lens[b] + i.  Slots with
-    lens[b] < 0 give zeros.  gate (optional): bf16 [B, M, HQ, D] view, out = bf16(o) * bf16(sigmoid(gate)) as in attn_decode_fused.
+    share (pages prefix_table [P] int32; prefix_len: an int, or a device integer, whose call is planned for all pages of
+    prefix_table: give it those in use, PagedState.prefix_pages) and its own rows <= lens[b] + i.  Slots with lens[b] < 0 give zeros.
+    Softmax weights meet V as bf16 over a bf16 pool, as f16 or hi + lo e4m3 over an e4m3 pool; everything else is held in fp32.  gate (optional): bf16 [B, M, HQ, D] view, out = bf16(o) * bf16(sigmoid(gate)) as in attn_decode_fused.
     Returns [B, M, HQ, D].  Lengths are read on the device, so a captured step serves all of them."""
     return (L._native or L.native()).attn_paged(q, k_pages, v_pages, table, lens, k_scale, v_scale, prefix_table, prefix_len, gate, scale, out)
 
