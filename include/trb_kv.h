@@ -329,7 +329,8 @@ int trb_paged_append(const trb_paged_t *pool, const trb_batch_t *batch, const tr
  * and its own rows <= lens[b] + i.  A prefix that pays for it is read once for the whole batch, on the tensor
  * cores.  Scores, sums and accumulators are fp32; softmax weights enter the product with V rounded: to bf16 over a bf16 pool, over an
  * e4m3 pool to f16 (off by 2^-25 of a row's largest weight where they are small) or, in the prefix's own kernel, to hi + lo e4m3 (8 bits;
- * off by 2^-16 of the largest weight among 128 neighbouring keys where they are small).  New rows should be finite: a non-finite V row can reach the sequence's earlier rows of the same step.
+ * off by 2^-16 of the largest weight among 128 neighbouring keys where they are small).
+ * New rows should be finite: a non-finite V row can reach the sequence's earlier rows of the same step.
  * Rows of the pool that no query sees may hold anything.  (hq / hkv) * m <= 128. */
 typedef struct trb_attn_paged_args {
     const void *q;               /* [n_seqs, m, hq, d] bf16                                     */

@@ -53,7 +53,8 @@ template <int D_, bool FP8_> struct PrefixCfg {
     // 65536 rows 265 -> 245 us).  e4m3 weights as hi + lo keep 8 bits down to 2^-10 of the reference and are off by up to 2^-18 of it below, so a
     // tail far under the largest weight would be lost whatever its mass: the reference also comes down, to within DROP bits of every
     // tile's own largest score.  What the small weights of a tile lose is then at most 128 * 2^-18 * 2^DROP = 2^-9 of its largest, however many keys there
-    // are (one sink and 65535 keys 18.5 bits below, a piece over all of them: off by 23 % -> 0.4 %; chats 40.4 -> 40.6 us, 128 readers of 65536 rows 230 -> 239, 512 934 -> 1021).
+    // are (one sink and 65535 keys 18.5 bits below, a piece over all of them: off by 23 % -> 0.4 %; 64 readers of 8192 rows 40.4 -> 40.6 us, 128 of 65536
+    // rows 230 -> 239, 512 query rows of 32/8 x 128 heads 934 -> 1021).
     // It stops DEPTH bits under the row's largest score, where a tile is worth nothing and O (<= keys * 448 * 2^(LIFT + DEPTH)) still fits fp32.
     static constexpr float LIFT = FP8 ? 8.f : 0.f, SLACK = 8.f, DROP = 2.f, DEPTH = 40.f;
     static constexpr int TM_S = 0, TM_O = 256, TM_Q = FP8 ? 0 : (D == 256 ? 128 : 384);
@@ -202,11 +203,13 @@ paged_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
         // no copy is on its way when the CTA leaves, also after a wait that ran out
         for (int t = max(0, k_sent - STAGES); t < k_sent; ++t) mbar_drain(&k_full[t % STAGES], (t / STAGES) & 1);
         for (int t = max(0, v_sent - STAGES); t < v_sent; ++t) mbar_drain(&v_full[t % STAGES], (t / STAGES) & 1);
+        __syncwarp();
     } else if (warp == PX_WARPS + 1) {
         // ================================ MMA issuer: one thread ==================================
         // QK(0), QK(1), PV(0), QK(2), PV(1), ..: the pipe runs in order of issue, so QK(i + 2) overwrites the buffer that holds
         // P(i) only after PV(i) has read it
-        if (lane == 0 && n_tiles > 0) {
+        if (lane != 0) return;                                                     // (the block's last barrier counts the threads that are left)
+        if (n_tiles > 0) {
             const uint32_t q_tm = tmem + C::TM_Q;
             const uint32_t q_hi = smem_u32(smem), q_lo = q_hi + C::Q_BYTES;
             constexpr uint32_t IDESC_QK = FP8 ? umma_idesc_f8(PX_BM, BN, false, false) : umma_idesc_bf16(PX_BM, BN, false, false);

@@ -358,7 +358,8 @@ def attn_paged(q, k_pages, v_pages, table, lens, k_scale=None, v_scale=None, *, 
     appended, lens is still the length before them).  Row i of sequence b sees the prefix_len rows that all sequences
     share (pages prefix_table [P] int32; prefix_len: an int, or a device integer, whose call is planned for all pages of
     prefix_table: give it those in use, PagedState.prefix_pages) and its own rows <= lens[b] + i.  Slots with lens[b] < 0 give zeros.
-    Softmax weights meet V as bf16 over a bf16 pool, as f16 or hi + lo e4m3 over an e4m3 pool; everything else is held in fp32.  gate (optional): bf16 [B, M, HQ, D] view, out = bf16(o) * bf16(sigmoid(gate)) as in attn_decode_fused.
+    Softmax weights meet V as bf16 over a bf16 pool, as f16 or hi + lo e4m3 over an e4m3 pool; everything else is held in fp32.
+    gate (optional): bf16 [B, M, HQ, D] view, out = bf16(o) * bf16(sigmoid(gate)) as in attn_decode_fused.
     Returns [B, M, HQ, D].  Lengths are read on the device, so a captured step serves all of them."""
     return (L._native or L.native()).attn_paged(q, k_pages, v_pages, table, lens, k_scale, v_scale, prefix_table, prefix_len, gate, scale, out)
 
